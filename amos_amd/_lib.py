@@ -5,7 +5,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libamos_mi355x.so")
 
-AMOS_F16, AMOS_BF16, AMOS_I8, AMOS_F32, AMOS_I32 = range(5)
+AMOS_F16, AMOS_BF16, AMOS_I8, AMOS_F32, AMOS_I32, AMOS_MXFP4 = range(6)
 AMOS_OP_GEMM, AMOS_OP_BGEMM, AMOS_OP_CONV2D, AMOS_OP_CONV3D = range(4)
 
 AMOS_PIPE_AUTO, AMOS_PIPE_STAGED, AMOS_PIPE_DIRECT4, AMOS_PIPE_DIRECT8, AMOS_PIPE_PATCH, AMOS_PIPE_PATCH8, AMOS_PIPE_NCHW = range(7)
@@ -77,6 +77,27 @@ class EltwiseDesc(ctypes.Structure):
                 ("program", _i32 * 16), ("consts", ctypes.c_float * 4)]
 
 
+class Mxfp4Desc(ctypes.Structure):
+    _fields_ = [("rows", _i64), ("cols", _i64), ("dtype", _i32), ("axis", _i32)]
+
+
+class Mxfp4GemmDesc(ctypes.Structure):
+    _fields_ = [("M", _i64), ("N", _i64), ("K", _i64), ("a_dtype", _i32), ("out_dtype", _i32)]
+
+
+class Mxfp4Epilogue(ctypes.Structure):
+    _fields_ = [("bias", ctypes.c_void_p), ("add", ctypes.c_void_p), ("bias_dtype", _i32), ("add_dtype", _i32)]
+
+
+AMOS_ACT_NONE, AMOS_ACT_RELU, AMOS_ACT_SILU = range(3)
+
+
+class GroupNormDesc(ctypes.Structure):
+    _fields_ = [("N", _i64), ("C", _i64), ("D", _i64), ("H", _i64), ("W", _i64), ("groups", _i32),
+                ("activation", _i32), ("x_dtype", _i32), ("y_dtype", _i32), ("affine_dtype", _i32), ("layout", _i32),
+                ("eps", ctypes.c_float), ("reserved", _i32)]
+
+
 class ComputeC(ctypes.Structure):
     _fields_ = [("n_tokens", _i32), ("tokens", ctypes.POINTER(_i32)), ("n_iters", _i32),
                 ("iter_kinds", ctypes.POINTER(_i32)), ("iter_extents", ctypes.POINTER(_i64)),
@@ -98,7 +119,9 @@ EXPORTS = [
     "amos_check_config", "amos_workspace_bytes", "amos_estimate_seconds", "amos_gemm", "amos_bgemm", "amos_conv2d",
     "amos_conv3d", "amos_conv2d_noalloc", "amos_conv_packed_weights_bytes", "amos_conv_pack_weights", "amos_run_fused", "amos_time", "amos_time_fused", "amos_gather", "amos_time_gather",
     "amos_eltwise", "amos_time_eltwise", "amos_kernel_name", "amos_match", "amos_enumerate_mappings",
-    "amos_mfma_ceiling",
+    "amos_mfma_ceiling", "amos_mxfp4_pitch", "amos_mxfp4_quantize", "amos_mxfp4_dequantize",
+    "amos_mxfp4_gemm_workspace_bytes", "amos_mxfp4_gemm", "amos_group_norm_workspace_bytes", "amos_group_norm",
+    "amos_group_norm_backward",
 ]
 
 _lib = None
@@ -162,6 +185,18 @@ def load():
     lib.amos_enumerate_mappings.argtypes = [_i32, _i32, ctypes.POINTER(_i32), ctypes.POINTER(_i64),
                                             ctypes.POINTER(_i64), ctypes.POINTER(ctypes.c_uint8),
                                             ctypes.POINTER(ctypes.c_uint8), _i32]
+    lib.amos_mxfp4_pitch.argtypes = [_i64]
+    lib.amos_mxfp4_pitch.restype = _i64
+    lib.amos_mxfp4_quantize.argtypes = [ctypes.POINTER(Mxfp4Desc), vp, vp, vp, vp]
+    lib.amos_mxfp4_dequantize.argtypes = [ctypes.POINTER(Mxfp4Desc), vp, vp, vp, vp]
+    lib.amos_mxfp4_gemm_workspace_bytes.argtypes = [ctypes.POINTER(Mxfp4GemmDesc)]
+    lib.amos_mxfp4_gemm_workspace_bytes.restype = sz
+    lib.amos_mxfp4_gemm.argtypes = [ctypes.POINTER(Mxfp4GemmDesc), ctypes.POINTER(Mxfp4Epilogue), vp, vp, vp, vp, vp,
+                                    vp, sz, vp]
+    lib.amos_group_norm_workspace_bytes.argtypes = [ctypes.POINTER(GroupNormDesc), ctypes.c_int]
+    lib.amos_group_norm_workspace_bytes.restype = sz
+    lib.amos_group_norm.argtypes = [ctypes.POINTER(GroupNormDesc), vp, vp, vp, vp, vp, vp, vp, sz, vp]
+    lib.amos_group_norm_backward.argtypes = [ctypes.POINTER(GroupNormDesc), vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, vp]
     _lib = lib
     return lib
 

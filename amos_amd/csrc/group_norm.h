@@ -1,0 +1,121 @@
+// Group norm with an activation over channels-last tensors, and its gradient, for gfx950.
+//
+//   per image n and group g of C / groups channels, over its pixels and channels:
+//     mean, var = E[x], E[(x - mean)^2];  h = (x - mean) / sqrt(var + eps)
+//     z = h weight[c] + bias[c];  y = act(z),  act none, relu or silu (z / (1 + exp(-z)))
+//   gradient, with d = dy act'(z):
+//     dweight[c] = sum d h,  dbias[c] = sum d      (over images and pixels)
+//     dx = (d weight - E[d weight] - h E[d weight h]) / sqrt(var + eps)   (E over the group)
+//
+// Both move bytes: a launch reads the tensors once for the sums, a second one reads them again and
+// writes.  A workgroup takes a run of pixels ("chunk") and a tile of channels; a lane keeps VEC
+// neighbouring channels and strides over pixels, so that a wave's loads are whole rows.  Sums are
+// joined in a fixed order (no atomics: the same bits on every run).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "dense_type.h"
+#include "fast_div.h"
+
+namespace amos {
+
+constexpr int kGnThreads = 256;
+
+struct GnParams {
+  const void* x;
+  const void* dy;            // gradient only
+  void* out;                 // y, dx
+  const void* weight;        // [C] or null (ones), of type affine_dtype
+  const void* bias;          // [C] or null (zeros)
+  float* mean;               // [N][G]: written by the forward launch, read by the gradient
+  float* rstd;
+  float* dweight;            // [C] or null
+  float* dbias;
+  float* part;               // workspace: see GnPlan
+  float* cpart;
+  int64_t image, pixel;      // elements between images, between pixels
+  int N, P, C, G, cpg;       // pixels of an image, channels, groups, channels of a group
+  int ct, tiles, sub;        // channels of a tile, tiles, tiles of a group (1 where a tile holds whole groups)
+  int cols, rows;            // threads across a tile's channels, pixels side by side
+  int chunk, chunks;         // pixels of a chunk, chunks of an image
+  int slots;                 // partial results of a group: chunks * sub
+  float eps;
+  int act, affine_dtype;
+  FastDiv by_cpg, by_cols;
+};
+
+// sums over the pixels of one group are kept as (count, mean, sum of squared deviations): no
+// difference of large sums, whatever the mean is
+struct GnStat {
+  float n, mean, m2;
+};
+
+__device__ __forceinline__ float gn_silu_factor(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+__device__ __forceinline__ float gn_act(float z, int act) {
+  if (act == AMOS_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
+  if (act == AMOS_ACT_SILU) return z * gn_silu_factor(z);
+  return z;
+}
+// dy act'(z)
+__device__ __forceinline__ float gn_act_gradient(float dy, float z, int act) {
+  if (act == AMOS_ACT_RELU) return z > 0.f ? dy : 0.f;
+  if (act == AMOS_ACT_SILU) {
+    const float s = gn_silu_factor(z);
+    return dy * (s * (1.f + z * (1.f - s)));
+  }
+  return dy;
+}
+
+// where a workgroup works
+struct GnTile {
+  int n, chunk, tile, c0, width;   // image, chunk, tile, first channel and channels of the tile
+  int g0, groups;                  // first group, groups the tile meets
+  int p0, p1;                      // pixels
+  int col, row;                    // of this thread
+  bool active;
+};
+template <int VEC>
+__device__ __forceinline__ GnTile gn_tile(const GnParams& p, int block) {
+  GnTile w;
+  w.tile = blockIdx.y;
+  w.n = block / p.chunks;
+  w.chunk = block - w.n * p.chunks;
+  w.c0 = w.tile * p.ct;
+  if (p.sub > 1) {   // tiles inside a group: the last of a group may be narrower
+    w.g0 = w.tile / p.sub;
+    const int s = w.tile - w.g0 * p.sub;
+    w.c0 = w.g0 * p.cpg + s * p.ct;
+    w.width = p.cpg - s * p.ct < p.ct ? p.cpg - s * p.ct : p.ct;
+    w.groups = 1;
+  } else {
+    w.g0 = w.c0 / p.cpg;
+    w.width = p.C - w.c0 < p.ct ? p.C - w.c0 : p.ct;
+    w.groups = w.width / p.cpg;
+  }
+  w.p0 = w.chunk * p.chunk;
+  w.p1 = w.p0 + p.chunk < p.P ? w.p0 + p.chunk : p.P;
+  const int t = threadIdx.x;
+  w.row = fast_div(t, p.by_cols);
+  w.col = t - w.row * p.cols;
+  w.active = w.row < p.rows && w.col * VEC < w.width;
+  return w;
+}
+
+// threads that share a group of a tile: a power of two inside a wave
+__device__ __forceinline__ int gn_team(int groups) {
+  int team = 64;
+  while (team > 1 && team * groups > kGnThreads) team >>= 1;
+  return team;
+}
+__device__ __forceinline__ float gn_team_sum(float v, int team) {
+  for (int s = 1; s < team; s <<= 1) v += __shfl_xor(v, s, 64);
+  return v;
+}
+
+struct GnPlan {
+  int vec;
+  int64_t part_floats, cpart_floats;
+};
+
+}  // namespace amos

@@ -461,6 +461,256 @@ def kernel_name(op, desc, config=None):
     return name.decode()
 
 
+class Mxfp4(object):
+    """A matrix [rows, cols] in microscaled 4 bits: blocks of 32 elements along a row share a
+    power-of-two scale.  `codes` uint8 [rows, 64 * ceil(cols / 128)], two e2m1 codes a byte (the element
+    of the lower index in the low half, zeros behind `cols`); `scales` uint8 [rows, codes' width / 16],
+    2^(byte - 127), 255 = not a number.  Where 128 divides `cols` there is no padding.  The tensors are
+    kept as they are, nothing is copied."""
+
+    __slots__ = ("codes", "scales", "shape")
+
+    def __init__(self, codes, scales, cols):
+        _need_device(codes, scales)
+        pitch = mxfp4_pitch(cols)
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+            raise ValueError("codes and scales are uint8, got %s and %s" % (codes.dtype, scales.dtype))
+        if codes.dim() != 2 or codes.shape[0] < 1 or codes.shape[1] != pitch or tuple(scales.shape) != (codes.shape[0], pitch // 16):
+            raise ValueError("%d columns want codes [rows, %d] and scales [rows, %d], got %s and %s"
+                             % (cols, pitch, pitch // 16, tuple(codes.shape), tuple(scales.shape)))
+        if codes.device != scales.device:
+            raise ValueError("codes are on %s, scales on %s" % (codes.device, scales.device))
+        self.codes, self.scales, self.shape = codes, scales, (codes.shape[0], int(cols))
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def __repr__(self):
+        return "Mxfp4(shape=%s, device=%s)" % (self.shape, self.device)
+
+
+def mxfp4_pitch(cols):
+    """bytes of a row of codes"""
+    if cols < 1:
+        raise ValueError("a matrix of %d columns" % cols)
+    return (int(cols) + 127) // 128 * 64
+
+
+_FLOAT_CODE = {torch.float32: _lib.AMOS_F32, torch.float16: _lib.AMOS_F16, torch.bfloat16: _lib.AMOS_BF16}
+
+
+def _float_code(what, dtype):
+    code = _FLOAT_CODE.get(dtype)
+    if code is None:
+        raise ValueError("%s is fp32, fp16 or bf16, got %s" % (what, dtype))
+    return code
+
+
+class _on(object):
+    """The device of a call's tensors made the current one, and the stream it launches on made
+    current there, so that what the call allocates belongs to that stream's pool."""
+
+    __slots__ = ("guards",)
+
+    def __init__(self, device, stream):
+        self.guards = []
+        if device.index != torch.cuda.current_device():
+            self.guards.append(torch.cuda.device(device))
+        if stream is not None:
+            if stream.device != device:
+                raise ValueError("the stream belongs to %s, the tensors are on %s" % (stream.device, device))
+            self.guards.append(torch.cuda.stream(stream))
+
+    def __enter__(self):
+        for g in self.guards:
+            g.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        for g in reversed(self.guards):
+            g.__exit__(*exc)
+        return False
+
+
+def _scratch(need, device):
+    """device scratch from the current stream's pool: (tensor, 256-byte aligned pointer)"""
+    ws = torch.empty(need + 255, dtype=torch.uint8, device=device)
+    return ws, (ws.data_ptr() + 255) // 256 * 256
+
+
+def _like_check(what, t, shape, device):
+    _need_device(t)
+    if tuple(t.shape) != tuple(shape) or t.device != device:
+        raise ValueError("%s must be of shape %s on %s, got %s on %s" % (what, tuple(shape), device, tuple(t.shape), t.device))
+
+
+def mxfp4_quantize(x, axis=1, out=None, stream=None):
+    """x [rows, cols] (fp32, fp16, bf16) -> Mxfp4.  axis 1: blocks along the rows, shape (rows, cols);
+    axis 0: blocks down the columns, the result is the quantised transpose, shape (cols, rows) -- what a
+    product that sums over the rows of x takes.  A block's scale brings its largest magnitude into
+    [4, 8); elements are rounded to nearest even and saturate at 6; a block with an infinity or a NaN
+    stands for NaN."""
+    _need_device(x)
+    if x.dim() != 2 or x.numel() == 0:
+        raise ValueError("x must be a matrix with elements, got shape %s" % (tuple(x.shape),))
+    if axis not in (0, 1, -1, -2):
+        raise ValueError("axis %s of a matrix" % (axis,))
+    axis = axis % 2
+    code = _float_code("x", x.dtype)
+    rows, cols = x.shape if axis else (x.shape[1], x.shape[0])
+    if out is not None and (not isinstance(out, Mxfp4) or out.shape != (rows, cols) or out.device != x.device):
+        raise ValueError("out must be an Mxfp4 of shape %s on %s, got %r" % ((rows, cols), x.device, out))
+    with _on(x.device, stream) as s:
+        if out is None:
+            pitch = mxfp4_pitch(cols)
+            out = Mxfp4(torch.empty((rows, pitch), dtype=torch.uint8, device=x.device),
+                        torch.empty((rows, pitch // 16), dtype=torch.uint8, device=x.device), cols)
+        d = _lib.Mxfp4Desc(x.shape[0], x.shape[1], code, axis)
+        check(_lib.load().amos_mxfp4_quantize(ctypes.byref(d), x.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), s))
+    return out
+
+
+def mxfp4_dequantize(q, dtype=torch.float32, out=None, stream=None):
+    """the values an Mxfp4 stands for, rounded once to `dtype` (fp32 and bf16 hold them all)"""
+    if not isinstance(q, Mxfp4):
+        raise ValueError("q must be an Mxfp4, got %s" % type(q))
+    if out is not None:
+        _need_device(out)
+        _check_out(out, q.shape, dtype, q.codes)
+    code = _float_code("the result", dtype)
+    with _on(q.device, stream) as s:
+        if out is None:
+            out = torch.empty(q.shape, dtype=dtype, device=q.device)
+        d = _lib.Mxfp4Desc(q.shape[0], q.shape[1], code, 1)
+        check(_lib.load().amos_mxfp4_dequantize(ctypes.byref(d), q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), s))
+    return out
+
+
+def mxfp4_gemm(a, b, out=None, out_dtype=torch.float32, add=None, bias=None, stream=None):
+    """C[M,N] = sum_k A(m,k) B(n,k) (+ bias[N]) (+ add[M,N]); b is an Mxfp4 of shape (N, K), a an
+    Mxfp4 of shape (M, K) or a dense matrix [M, K] (fp32, fp16, bf16) that the call quantises the way
+    mxfp4_quantize does.  fp32 accumulation, one rounding to the output's type; `add` may be `out`."""
+    if not isinstance(b, Mxfp4):
+        raise ValueError("b must be an Mxfp4, got %s" % type(b))
+    dense = not isinstance(a, Mxfp4)
+    if dense:
+        _need_device(a)
+        a_code = _float_code("a", a.dtype)
+    else:
+        a_code = _lib.AMOS_MXFP4
+    if len(a.shape) != 2 or a.shape[0] < 1 or a.shape[1] != b.shape[1] or a.device != b.device:
+        raise ValueError("operands do not agree: a %s on %s, b %s on %s" % (tuple(a.shape), a.device, b.shape, b.device))
+    M, N, K = a.shape[0], b.shape[0], b.shape[1]
+    if out is not None:
+        out_dtype = out.dtype
+        _like_check("out", out, (M, N), b.device)
+    d = _lib.Mxfp4GemmDesc(M, N, K, a_code, _float_code("the output", out_dtype))
+    epi = None
+    if add is not None or bias is not None:
+        epi = _lib.Mxfp4Epilogue()
+        if bias is not None:
+            _like_check("bias", bias, (N,), b.device)
+            epi.bias, epi.bias_dtype = bias.data_ptr(), _float_code("bias", bias.dtype)
+        if add is not None:
+            _like_check("the added operand", add, (M, N), b.device)
+            epi.add, epi.add_dtype = add.data_ptr(), _float_code("the added operand", add.dtype)
+    lib = _lib.load()
+    with _on(b.device, stream) as s:
+        if out is None:
+            out = torch.empty((M, N), dtype=out_dtype, device=b.device)
+        need = lib.amos_mxfp4_gemm_workspace_bytes(ctypes.byref(d))
+        ws, ws_ptr = _scratch(need, b.device) if need else (None, None)
+        ac, asc = (a.data_ptr(), None) if dense else (a.codes.data_ptr(), a.scales.data_ptr())
+        check(lib.amos_mxfp4_gemm(ctypes.byref(d), None if epi is None else ctypes.byref(epi), ac, asc, b.codes.data_ptr(),
+                                  b.scales.data_ptr(), out.data_ptr(), ws_ptr, need, s))
+    return out
+
+
+_ACT_CODE = {None: _lib.AMOS_ACT_NONE, "none": _lib.AMOS_ACT_NONE, "relu": _lib.AMOS_ACT_RELU, "silu": _lib.AMOS_ACT_SILU}
+
+
+def _group_norm_desc(x, groups, weight, bias, eps, activation, layout, out_dtype):
+    code = _lib.LAYOUT_CODE.get(layout)
+    if code not in (_lib.AMOS_LAYOUT_NHWC, _lib.AMOS_LAYOUT_HWNC):
+        raise ValueError("group norm runs on the channels-last layouts (nhwc, ndhwc, hwnc, dhwnc), got %r" % (layout,))
+    if x.dim() != len(layout) or x.numel() == 0:
+        raise ValueError("layout %s wants a tensor of %d dimensions with elements, got shape %s" % (layout, len(layout), tuple(x.shape)))
+    if activation not in _ACT_CODE:
+        raise ValueError("activation is None, 'relu' or 'silu', got %r" % (activation,))
+    ext = dict(zip(layout, x.shape))
+    if groups < 1 or ext["c"] % groups:
+        raise ValueError("%d channels in %d groups" % (ext["c"], groups))
+    d = _lib.GroupNormDesc()
+    d.N, d.C, d.D, d.H, d.W = ext["n"], ext["c"], ext.get("d", 1), ext["h"], ext["w"]
+    d.groups, d.activation, d.layout, d.eps = groups, _ACT_CODE[activation], code, eps
+    d.x_dtype, d.y_dtype = _float_code("x", x.dtype), _float_code("the output", out_dtype)
+    for what, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _like_check(what, t, (ext["c"],), x.device)
+            d.affine_dtype = _float_code(what, t.dtype)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight is %s, bias %s" % (weight.dtype, bias.dtype))
+    return d
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, layout="nhwc", out_dtype=None, out=None,
+               stats=False, stream=None):
+    """act(group norm of x) over a channels-last tensor (layout nhwc, ndhwc, hwnc or dhwnc): per image
+    and group of neighbouring channels h = (x - mean) / sqrt(var + eps), then h * weight[C] + bias[C],
+    then None / 'relu' / 'silu'.  Statistics and arithmetic are fp32, the result is x's type or
+    out_dtype (a convolution's fp32 output can leave at 16 bits for the next one); `out` may be x.
+    stats=True: (y, mean, rstd), both fp32 [N, groups], for group_norm_backward."""
+    _need_device(x)
+    if out is not None:
+        _like_check("out", out, x.shape, x.device)
+        if out_dtype is not None and out_dtype != out.dtype:
+            raise ValueError("out is %s, out_dtype %s" % (out.dtype, out_dtype))
+        out_dtype = out.dtype
+    elif out_dtype is None:
+        out_dtype = x.dtype
+    d = _group_norm_desc(x, groups, weight, bias, eps, activation, layout, out_dtype)
+    lib = _lib.load()
+    with _on(x.device, stream) as s:
+        if out is None:
+            out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
+        mean = rstd = None
+        if stats:
+            mean, rstd = torch.empty((2, d.N, groups), dtype=torch.float32, device=x.device).unbind(0)
+        need = lib.amos_group_norm_workspace_bytes(ctypes.byref(d), 0)
+        ws, ws_ptr = _scratch(need, x.device) if need else (None, None)
+        check(lib.amos_group_norm(ctypes.byref(d), x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), _ptr(mean), _ptr(rstd),
+                                  ws_ptr, need, s))
+    return (out, mean, rstd) if stats else out
+
+
+def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, activation=None, layout="nhwc", stream=None):
+    """gradients of group_norm: (dx of x's type, dweight, dbias in fp32 -- None where the coefficient
+    is), from the statistics that group_norm(..., stats=True) returned for x"""
+    _need_device(dy, x, mean, rstd)
+    if dy.shape != x.shape or dy.device != x.device:
+        raise ValueError("dy is %s on %s, x %s on %s" % (tuple(dy.shape), dy.device, tuple(x.shape), x.device))
+    d = _group_norm_desc(x, groups, weight, bias, 0.0, activation, layout, dy.dtype)
+    for what, t in (("mean", mean), ("rstd", rstd)):
+        _like_check(what, t, (d.N, groups), x.device)
+        if t.dtype != torch.float32:
+            raise ValueError("%s is fp32, got %s" % (what, t.dtype))
+    lib = _lib.load()
+    with _on(x.device, stream) as s:
+        dx = torch.empty_like(x)
+        dweight = None if weight is None else torch.empty(d.C, dtype=torch.float32, device=x.device)
+        dbias = None if bias is None else torch.empty(d.C, dtype=torch.float32, device=x.device)
+        need = lib.amos_group_norm_workspace_bytes(ctypes.byref(d), 1)
+        ws, ws_ptr = _scratch(need, x.device) if need else (None, None)
+        check(lib.amos_group_norm_backward(ctypes.byref(d), dy.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias), mean.data_ptr(),
+                                           rstd.data_ptr(), dx.data_ptr(), _ptr(dweight), _ptr(dbias), ws_ptr, need, s))
+    return dx, dweight, dbias
+
+
 def device_info():
     info = _lib.DeviceInfo()
     check(_lib.load().amos_device_info(ctypes.byref(info)))

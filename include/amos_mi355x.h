@@ -50,7 +50,8 @@ typedef enum {
   AMOS_BF16 = 1,
   AMOS_I8 = 2,
   AMOS_F32 = 3,
-  AMOS_I32 = 4
+  AMOS_I32 = 4,
+  AMOS_MXFP4 = 5   /* microscaled 4 bits: operands of amos_mxfp4_gemm only */
 } amos_dtype_t;
 
 typedef enum {
@@ -359,6 +360,97 @@ int amos_time_eltwise(const amos_eltwise_desc_t* desc, const void* const* inputs
 int amos_mfma_ceiling(int shape, int random_operands, int copies, int reads, const void* a, const void* b,
                       size_t operand_bytes, void* sink, int launches, void* stream, double* out_seconds,
                       double* out_flop);
+
+/* ---- microscaled 4-bit matrices --------------------------------------------------------------- */
+
+/*
+ * Blocks of 32 consecutive elements of a row share a power-of-two scale:
+ *   codes   [rows][pitch] bytes, pitch = amos_mxfp4_pitch(cols) = 64 * ceil(cols / 128): two e2m1
+ *           codes a byte, the element of the lower index in the low half; elements behind `cols` are
+ *           zeros.  16-byte aligned.
+ *   scales  [rows][pitch / 16] bytes, a block's scale is 2^(byte - 127), 255 = not a number; bytes
+ *           behind the last block are 0.  4-byte aligned.
+ * Quantisation: for a block with largest magnitude m the scale is 2^e, e = max(floor(log2 m) - 2,
+ * -127) (an all-zero block: -127); every element / 2^e is rounded to the nearest of 0, 1/2, 1, 3/2,
+ * 2, 3, 4, 6 (ties to the even code), magnitudes above 6 become 6.  A block that holds an infinity
+ * or a NaN gets the scale byte 255 and codes of 0, and stands for NaN.
+ *   axis = 1: x [rows][cols] -> quantised [rows][cols]
+ *   axis = 0: blocks run down the columns of x, the result is the quantised TRANSPOSE [cols][rows]
+ *             (what a product that sums over the rows of x takes: the two products of a layer's
+ *             backward pass)
+ * x is dense, fp32, fp16 or bf16.  The reference has no microscaled type.
+ */
+typedef struct {
+  int64_t rows, cols;   /* of the dense matrix */
+  int32_t dtype;        /* AMOS_F32 / AMOS_F16 / AMOS_BF16 */
+  int32_t axis;         /* quantisation: 0 or 1; dequantisation: 1 */
+} amos_mxfp4_desc_t;
+
+int64_t amos_mxfp4_pitch(int64_t cols);
+int amos_mxfp4_quantize(const amos_mxfp4_desc_t* desc, const void* x, void* codes, void* scales, void* stream);
+/* the values of codes [rows][cols] in desc->dtype (rounded to it once) */
+int amos_mxfp4_dequantize(const amos_mxfp4_desc_t* desc, const void* codes, const void* scales, void* out, void* stream);
+
+/*
+ * C[m][n] = sum_k A[m][k] B[n][k] (+ bias[n]) (+ D[m][n]): both operands microscaled 4-bit matrices
+ * with K along their rows, fp32 accumulation, one rounding to the output type.  C and D are dense
+ * [M][N].  a_dtype AMOS_MXFP4: A is codes, a_scales its scales.  a_dtype fp32 / fp16 / bf16: A is a
+ * dense matrix [M][K] that the call quantises (axis 1) before it multiplies; a_scales is not read.
+ * D may be C where its type is C's.
+ */
+typedef struct {
+  int64_t M, N, K;
+  int32_t a_dtype;     /* AMOS_MXFP4 / AMOS_F32 / AMOS_F16 / AMOS_BF16 */
+  int32_t out_dtype;   /* AMOS_F32 / AMOS_F16 / AMOS_BF16 */
+} amos_mxfp4_gemm_desc_t;
+typedef struct {
+  const void* bias;    /* device pointer, [N], or NULL */
+  const void* add;     /* device pointer, [M][N], or NULL */
+  int32_t bias_dtype, add_dtype;   /* AMOS_F32 / AMOS_F16 / AMOS_BF16 */
+} amos_mxfp4_epilogue_t;
+
+/* bytes of 256-byte aligned device scratch the call wants; less: AMOS_ERR_WORKSPACE */
+size_t amos_mxfp4_gemm_workspace_bytes(const amos_mxfp4_gemm_desc_t* desc);
+int amos_mxfp4_gemm(const amos_mxfp4_gemm_desc_t* desc, const amos_mxfp4_epilogue_t* epilogue, const void* A,
+                    const void* a_scales, const void* B, const void* b_scales, void* C, void* workspace,
+                    size_t ws_bytes, void* stream);
+
+/* ---- group norm with an activation, channels last ---------------------------------------------- */
+
+/*
+ * Per image n and group of C / groups neighbouring channels, over its D*H*W pixels and channels:
+ *   mean = E[x], var = E[(x - mean)^2], h = (x - mean) / sqrt(var + eps), y = act(h weight[c] + bias[c])
+ * x, y (dy, dx) are dense in one of the channels-last layouts of the convolutions (AMOS_LAYOUT_NHWC,
+ * AMOS_LAYOUT_HWNC); weight, bias [C] of one type, or NULL (ones, zeros).  Arithmetic and statistics
+ * are fp32; mean and rstd = 1 / sqrt(var + eps) are written as fp32 [N][groups] where not NULL.  y may
+ * be x where their types agree.
+ * Gradient (with the forward's mean and rstd): dx of x's type, dweight and dbias fp32 [C] or NULL; dy has
+ * y's type.  dx may be dy or x where the types agree.  Results do not depend on the order in which
+ * workgroups run.
+ * The reference leaves normalisation layers to its fallback scheduler
+ * (python/tvm/tensor_graph/core/auto_schedule/auto_schedule.py:1090-1160).
+ */
+#define AMOS_ACT_NONE 0
+#define AMOS_ACT_RELU 1
+#define AMOS_ACT_SILU 2   /* z / (1 + exp(-z)) */
+typedef struct {
+  int64_t N, C, D, H, W;
+  int32_t groups;
+  int32_t activation;             /* AMOS_ACT_* */
+  int32_t x_dtype, y_dtype;       /* AMOS_F32 / AMOS_F16 / AMOS_BF16 */
+  int32_t affine_dtype;           /* of weight and bias */
+  int32_t layout;                 /* AMOS_LAYOUT_NHWC / AMOS_LAYOUT_HWNC */
+  float eps;
+  int32_t reserved;
+} amos_group_norm_desc_t;
+
+/* bytes of device scratch the call wants; less: AMOS_ERR_WORKSPACE */
+size_t amos_group_norm_workspace_bytes(const amos_group_norm_desc_t* desc, int gradient);
+int amos_group_norm(const amos_group_norm_desc_t* desc, const void* x, const void* weight, const void* bias,
+                    void* y, float* mean, float* rstd, void* workspace, size_t ws_bytes, void* stream);
+int amos_group_norm_backward(const amos_group_norm_desc_t* desc, const void* dy, const void* x, const void* weight,
+                             const void* bias, const float* mean, const float* rstd, void* dx, float* dweight,
+                             float* dbias, void* workspace, size_t ws_bytes, void* stream);
 
 /* name of the kernel instance a (desc, cfg) pair dispatches to, e.g.
  * "amos_igemm<f16,vec,vec,256x256>"; replaces func.imported_modules[0].get_source()
