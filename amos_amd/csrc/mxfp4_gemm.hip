@@ -2,7 +2,10 @@
 
 #include <string.h>
 
+#include <mutex>
+
 #include "mapper.h"
+#include "mxfp4_tile_kernel.h"
 
 namespace amos {
 
@@ -141,6 +144,37 @@ static void launch_few(const MxGemmParams& p, int src, hipStream_t stream) {
   else hipLaunchKernelGGL((amos_mx_gemm_few<SRC_BF16, RT, TT>), grid, block, 0, stream, p);
 }
 
+// ---- many rows of A -----------------------------------------------------------------------------
+template <int WI, int WJ, int BI, int BJ, int NS>
+static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
+  constexpr int lds = NS * (BI + BJ) * 136;
+  void (*const fn)(const MxTileParams) = amos_mx_gemm_tile<WI, WJ, BI, BJ, NS>;
+  static std::once_flag once;
+  static hipError_t err = hipSuccess;
+  static int spilled = 0;
+  std::call_once(once, [&] {
+    err = hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    // (the kernel counts its outstanding copies; register spills would count among them)
+    hipFuncAttributes fa;
+    if (err == hipSuccess) err = hipFuncGetAttributes(&fa, (const void*)fn);
+    if (err == hipSuccess) spilled = (int)fa.localSizeBytes;
+  });
+  if (err != hipSuccess) return set_error(AMOS_ERR_HIP, "amos_mx_gemm_tile<%dx%d>: %s", BI, BJ, hipGetErrorString(err));
+  if (spilled) return set_error(AMOS_ERR_INFEASIBLE, "amos_mx_gemm_tile<%dx%d> was built with scratch memory", BI, BJ);
+  MxTileParams t;
+  t.g = p;
+  t.tiles_i = (p.M + BI - 1) / BI;
+  t.tiles_j = (p.N + BJ - 1) / BJ;
+  t.per_split = (p.steps + 1) / 2;
+  t.slices = nullptr;
+  const int es = dense_size(p.out_dtype);
+  t.vec_out = ((uintptr_t)p.c & 15) == 0 && ((int64_t)p.N * es) % 16 == 0;
+  t.vec_add = p.tail.add && ((uintptr_t)p.tail.add & 15) == 0;   // (N is a multiple of the run then)
+  if ((int64_t)t.tiles_i * t.tiles_j >= (int64_t)1 << 31) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d x %d results", p.M, p.N);
+  hipLaunchKernelGGL(fn, dim3((unsigned)(t.tiles_i * t.tiles_j), 1), dim3(64 * WI * WJ), lds, stream, t);
+  return 0;
+}
+
 int mx_quantize(const amos_mxfp4_desc_t* d, const void* x, void* codes, void* scales, hipStream_t stream);
 
 static int check_desc(const amos_mxfp4_gemm_desc_t* d) {
@@ -209,6 +243,15 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
   } else {
     p.a = (const unsigned char*)A;
     p.as = (const unsigned char*)a_scales;
+  }
+  // (the tiled kernel's offsets inside a tile have 32 bits)
+  if (d->M > 64 && p.steps < 1 << 18) {
+    const int64_t big = ((d->M + 255) / 256) * ((d->N + 255) / 256);
+    rc = big >= 256 ? launch_tile<2, 4, 256, 256, 2>(p, stream) : launch_tile<2, 4, 128, 128, 2>(p, stream);
+    if (rc) return rc;
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return set_error(AMOS_ERR_HIP, "launch failed: %s", hipGetErrorString(err));
+    return 0;
   }
   if ((d->M + 63) / 64 > 65535) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of more than %d rows", 65535 * 64);
   if (d->M <= 16) launch_few<1, 1>(p, src, stream);

@@ -1,0 +1,272 @@
+// Tiled product of two microscaled 4-bit matrices: many rows on both sides.
+//
+// Block tile BI x BJ, K step 256 elements = 128 bytes of every row, NS stages in LDS of
+// (BI + BJ) * 136 bytes: the codes as rows of eight 16-byte chunks (XOR-swizzled by row, the swizzle
+// applied on the global side), behind them eight scale bytes a row.  Both travel by direct copies
+// (global_load_lds, 16 and 4 bytes a lane); the copies of step t + NS leave right behind the one
+// barrier of step t.  A K step is two matrix instructions deep (K = 128 each) and each of them is
+// issued in two halves over the wave tile's rows, so that the fragments of the next half are read
+// while this one multiplies.  A fragment is one 16-byte LDS read and one byte read for its block's scale: the
+// byte arrives in the register the matrix instruction takes it from, no instruction touches it.
+// Rows past M / N repeat the last one (their sums are not stored).  K is padded to 128 by the format; an
+// odd number of 128s ends in a half step whose second half is neither read from memory (its lanes fetch
+// the first half again: the row may be the buffer's last) nor multiplied.
+#pragma once
+#include <type_traits>
+
+#include "igemm_kernel.h"
+#include "mxfp4_gemm.h"
+
+namespace amos {
+
+struct MxTileParams {
+  MxGemmParams g;
+  int tiles_i, tiles_j;
+  int per_split;        // K steps of a split (blockIdx.y); its sums go to `slices` + y * M * N, fp32
+  float* slices;        // null: not split
+  int vec_out;          // C's rows are whole 16-byte pieces
+  int vec_add;          // ... and D's can be read by the same pieces
+};
+
+// LDS place of a row's 16-byte chunk.  The swizzle goes by the row inside its block of 16, so that the fragments of
+// a wave's row blocks lie at constant distances; a fragment read (16 rows, chunks c and c + 2 in either half of the
+// wave) puts two lanes on every 16-byte slot of the 256-byte bank space, its minimum.
+__device__ __forceinline__ int mx_lds_offset(int row, int chunk) {
+  return row * 128 + ((chunk ^ ((row ^ ((row >> 3) & 1)) & 7)) << 4);
+}
+
+#define AMOS_MX_GLOBAL(p) ((const __attribute__((address_space(1))) void*)(p))
+#define AMOS_MX_LDS(p) ((__attribute__((address_space(3))) void*)(p))
+
+// V consecutive values of a dense tensor; `whole`: they are aligned to V elements (or 16 bytes)
+template <int V>
+__device__ __forceinline__ void mx_load_run(const void* p, int64_t at, int dtype, int whole, float* v) {
+  if (whole) {
+    if (dtype == AMOS_F32) {
+#pragma unroll
+      for (int i = 0; i < V; i += 4) DenseVec<TypeF32, 4>::load((const float*)p + at + i, v + i);
+    } else if (dtype == AMOS_F16) {
+      DenseVec<TypeF16, V>::load((const _Float16*)p + at, v);
+    } else {
+      DenseVec<TypeBF16, V>::load((const __bf16*)p + at, v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = load_any(p, at + i, dtype);
+  }
+}
+
+template <int WI, int WJ, int BI, int BJ, int NS>
+__global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTileParams t) {
+  constexpr int NW = WI * WJ;
+  constexpr int TI = BI / (16 * WI), TJ = BJ / (16 * WJ);
+  constexpr int HA = TI / 2;
+  static_assert(TI % 2 == 0 && TI * WI * 16 == BI && TJ * WJ * 16 == BJ && TJ >= 1, "wave tile");
+  constexpr int OPER = BI * 128, CODES = (BI + BJ) * 128, STAGE = (BI + BJ) * 136;
+  constexpr int QA = BI / 8;
+  constexpr int CH = (BI + BJ) / 8 / NW, SCH = (BI + BJ) / 32 / NW;
+  static_assert(CH >= 1 && CH * NW * 8 == BI + BJ && SCH >= 1 && SCH * NW * 32 == BI + BJ, "copies");
+  constexpr int COPIES = CH + SCH;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const MxGemmParams& p = t.g;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wi = wave / WJ, wj = wave % WJ;
+  int tile_i, tile_j;
+  block_to_tile(blockIdx.x, gridDim.x, t.tiles_i, t.tiles_j, tile_i, tile_j);
+  const int bi0 = tile_i * BI, bj0 = tile_j * BJ;
+  const int64_t pitch = (int64_t)p.steps * 64, spitch = (int64_t)p.steps * 4;
+  const int kt0 = (int)blockIdx.y * t.per_split;
+  const unsigned char* const abase = p.a + bi0 * pitch + (int64_t)kt0 * 128;
+  const unsigned char* const bbase = p.b + bj0 * pitch + (int64_t)kt0 * 128;
+  const unsigned char* const asbase = p.as + bi0 * spitch + (int64_t)kt0 * 8;
+  const unsigned char* const bsbase = p.bs + bj0 * spitch + (int64_t)kt0 * 8;
+  // this block's whole K steps, and whether a half one follows
+  int steps = p.steps - 2 * kt0;
+  if (steps > 2 * t.per_split) steps = 2 * t.per_split;
+  const int full = steps >> 1, half = steps & 1, KT = full + half;
+
+  unsigned g_off[CH], s_off[SCH];
+  const int chunk = (lane & 7) ^ (((lane >> 3) ^ (wave & 1)) & 7);   // (NW even: the same for every copy of the wave)
+  static_assert(NW % 2 == 0 && QA % 2 == 0, "one swizzle term per wave");
+#pragma unroll
+  for (int u = 0; u < CH; ++u) {
+    const int q = wave + NW * u;
+    const int row = (q < QA ? q : q - QA) * 8 + (lane >> 3);
+    const int r = q < QA ? (bi0 + row < p.M ? row : p.M - 1 - bi0) : (bj0 + row < p.N ? row : p.N - 1 - bj0);
+    g_off[u] = (unsigned)r * (unsigned)pitch + chunk * 16;
+  }
+#pragma unroll
+  for (int u = 0; u < SCH; ++u) {
+    const int row = (wave + NW * u) * 32 + (lane >> 1);
+    const int r = row < BI ? (bi0 + row < p.M ? row : p.M - 1 - bi0) : (bj0 + row - BI < p.N ? row - BI : p.N - 1 - bj0);
+    s_off[u] = (unsigned)r * (unsigned)spitch + (lane & 1) * 4;
+  }
+  const unsigned back = chunk >= 4 ? 64 : 0, sback = (lane & 1) * 4;   // what a half step's second half steps back
+  auto issue_copies = [&](int kt, int stage) {
+    const bool h = kt >= full;
+    const unsigned char *ak = abase + (int64_t)kt * 128 - (h ? back : 0u), *bk = bbase + (int64_t)kt * 128 - (h ? back : 0u);
+    const unsigned char *as = asbase + (int64_t)kt * 8 - (h ? sback : 0u), *bs = bsbase + (int64_t)kt * 8 - (h ? sback : 0u);
+    char* s = smem + stage * STAGE;
+#pragma unroll
+    for (int u = 0; u < CH; ++u) {
+      const int q = wave + NW * u;
+      __builtin_amdgcn_global_load_lds(AMOS_MX_GLOBAL((q < QA ? ak : bk) + g_off[u]), AMOS_MX_LDS(s + q * 1024), 16, 0, 0);
+    }
+#pragma unroll
+    for (int u = 0; u < SCH; ++u) {
+      const int q = wave + NW * u;
+      __builtin_amdgcn_global_load_lds(AMOS_MX_GLOBAL((q * 32 < BI ? as : bs) + s_off[u]), AMOS_MX_LDS(s + CODES + q * 256), 4, 0, 0);
+    }
+  };
+
+  // which of a sub-step's four blocks a lane group takes is free as long as both operands agree; groups q and
+  // q + 2 take neighbouring chunks, which the swizzle puts on different banks
+  const int frag_row = lane & 15, frag_q = lane >> 4;
+  const int frag_chunk = (frag_q >> 1) | ((frag_q & 1) << 1);
+  const int a_off = mx_lds_offset(wi * TI * 16 + frag_row, frag_chunk), b_off = OPER + mx_lds_offset(wj * TJ * 16 + frag_row, frag_chunk);
+  const int as_off = CODES + (wi * TI * 16 + frag_row) * 8 + frag_chunk, bs_off = CODES + (BI + wj * TJ * 16 + frag_row) * 8 + frag_chunk;
+
+  v4f acc[TI][TJ];
+#pragma unroll
+  for (int a = 0; a < TI; ++a)
+#pragma unroll
+    for (int b = 0; b < TJ; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
+
+  mx_v4i af[2][HA], bf[2][TJ];
+  int ax[2][HA], bx[2][TJ];
+  auto read_a = [&](int stage, int ks, int h, int slot) {
+    const char* s = smem + stage * STAGE;
+#pragma unroll
+    for (int a = 0; a < HA; ++a) {
+      const int ab = h * HA + a;
+      af[slot][a] = *(const mx_v4i*)(s + (a_off ^ (ks * 64)) + ab * 2048);
+      ax[slot][a] = *(const unsigned char*)(s + as_off + ab * 128 + ks * 4);
+    }
+  };
+  auto read_b = [&](int stage, int ks, int slot) {
+    const char* s = smem + stage * STAGE;
+#pragma unroll
+    for (int b = 0; b < TJ; ++b) {
+      bf[slot][b] = *(const mx_v4i*)(s + (b_off ^ (ks * 64)) + b * 2048);
+      bx[slot][b] = *(const unsigned char*)(s + bs_off + b * 128 + ks * 4);
+    }
+  };
+  auto mma = [&](int h, int sa, int sb) {
+#pragma unroll
+    for (int b = 0; b < TJ; ++b)
+#pragma unroll
+      for (int a = 0; a < HA; ++a) acc[h * HA + a][b] = mx_mfma(af[sa][a], bf[sb][b], acc[h * HA + a][b], ax[sa][a], bx[sb][b]);
+  };
+
+  static_assert(NS >= 2 && (NS - 1) * COPIES <= 63, "stages");
+#pragma unroll
+  for (int s = 0; s < NS; ++s) issue_copies(s < KT ? s : KT - 1, s);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * COPIES) : "memory");
+  read_a(0, 0, 0, 0);
+  read_b(0, 0, 0);
+
+  int st = 0;
+  for (int kt = 0; kt < full; ++kt) {
+    const int st_next = st + 1 == NS ? 0 : st + 1;
+    read_a(st, 0, 1, 1);
+    mma(0, 0, 0);
+    read_a(st, 1, 0, 0);
+    read_b(st, 1, 1);
+    mma(1, 1, 0);
+    read_a(st, 1, 1, 1);
+    mma(0, 0, 1);
+    // all reads of this stage are issued; once they and this wave's copies of the next tile are done, meet: behind
+    // the barrier the next stage is whole and this one is free
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * COPIES) : "memory");
+    issue_copies(kt + NS < KT ? kt + NS : KT - 1, st);
+    read_a(st_next, 0, 0, 0);   // (behind the last step: read and not used)
+    read_b(st_next, 0, 0);
+    mma(1, 1, 1);
+    st = st_next;
+  }
+  if (half) {
+    read_a(st, 0, 1, 1);
+    mma(0, 0, 0);
+    mma(1, 1, 0);
+  }
+
+  // ---- the sums leave through a strip of LDS per wave (half the wave tile's rows at a time): whole rows, 16 bytes
+  // a lane; bias and D join there, in fp32, before the one rounding
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // (the last copies have landed, all reads are done)
+  constexpr int SP = TJ * 16 + 4, SR = HA * 16;
+  static_assert(NW * SR * SP * 4 <= NS * STAGE, "output strip");
+  float* const strip = (float*)smem + wave * (SR * SP);
+  const bool split = t.slices != nullptr;
+  void* const out = split ? (void*)(t.slices + (int64_t)blockIdx.y * p.M * p.N) : p.c;
+  const int out_dtype = split ? (int)AMOS_F32 : p.out_dtype;
+  const int wj0 = bj0 + wj * TJ * 16;
+  // V neighbouring results of a lane
+  auto emit = [&](int i, int j, float* v, auto width) {
+    constexpr int V = decltype(width)::value;
+    const int64_t at = (int64_t)i * p.N + j;
+    float e[V];
+    if (!split && p.tail.bias) {
+      mx_load_run<V>(p.tail.bias, j, p.tail.bias_dtype, 0, e);
+#pragma unroll
+      for (int x = 0; x < V; ++x) v[x] += e[x];
+    }
+    if (!split && p.tail.add) {
+      mx_load_run<V>(p.tail.add, at, p.tail.add_dtype, t.vec_add, e);
+#pragma unroll
+      for (int x = 0; x < V; ++x) v[x] += e[x];
+    }
+    if constexpr (V == 4) {
+      DenseVec<TypeF32, 4>::store((float*)out + at, v);
+    } else {
+      if (out_dtype == AMOS_F16) DenseVec<TypeF16, 8>::store((_Float16*)out + at, v);
+      else DenseVec<TypeBF16, 8>::store((__bf16*)out + at, v);
+    }
+  };
+  auto store_half = [&](int h) {
+#pragma unroll
+    for (int a = 0; a < HA; ++a)
+#pragma unroll
+      for (int b = 0; b < TJ; ++b)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) strip[(a * 16 + 4 * frag_q + r) * SP + b * 16 + frag_row] = acc[h * HA + a][b][r];
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    const int i0 = bi0 + (wi * TI + h * HA) * 16;
+    if (t.vec_out && out_dtype == AMOS_F32) {
+      constexpr int LPR = TJ * 4, RPI = 64 / LPR;
+#pragma unroll 2
+      for (int n = 0; n < SR / RPI; ++n) {
+        const int row = n * RPI + lane / LPR, col = (lane % LPR) * 4;
+        float v[4];
+        DenseVec<TypeF32, 4>::load(strip + row * SP + col, v);
+        if (i0 + row < p.M && wj0 + col < p.N) emit(i0 + row, wj0 + col, v, std::integral_constant<int, 4>{});
+      }
+    } else if (t.vec_out) {
+      constexpr int LPR = TJ * 2, RPI = 64 / LPR;
+      static_assert(SR % RPI == 0, "strip rows");
+#pragma unroll 2
+      for (int n = 0; n < SR / RPI; ++n) {
+        const int row = n * RPI + lane / LPR, col = (lane % LPR) * 8;
+        float v[8];
+        DenseVec<TypeF32, 4>::load(strip + row * SP + col, v);
+        DenseVec<TypeF32, 4>::load(strip + row * SP + col + 4, v + 4);
+        if (i0 + row < p.M && wj0 + col < p.N) emit(i0 + row, wj0 + col, v, std::integral_constant<int, 8>{});
+      }
+    } else {
+      for (int e = lane; e < SR * TJ * 16; e += 64) {
+        const int row = e / (TJ * 16), col = e % (TJ * 16);
+        const int i = i0 + row, j = wj0 + col;
+        if (i < p.M && j < p.N) {
+          float v = strip[row * SP + col];
+          if (!split) v = mx_tail(p.tail, v, i, j, p.N);
+          store_any(out, (int64_t)i * p.N + j, out_dtype, v);
+        }
+      }
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the strip is read before it is written again)
+  };
+  store_half(0);
+  store_half(1);
+}
+
+}  // namespace amos

@@ -175,7 +175,7 @@ def resources(log_text):
 # (s_waitcnt vmcnt(n), n > 0): a register spill's scratch access counts on the same counter, so a
 # spilling instance would wait for the wrong accesses.  The build refuses such an instance; the
 # library refuses to launch one as well (amos_runtime.hip: launch_tn, launch_conv).
-NO_SCRATCH = ("amos_gemm_tn", "amos_conv_fprop", "amos_conv_nchw")
+NO_SCRATCH = ("amos_gemm_tn", "amos_conv_fprop", "amos_conv_nchw", "amos_mx_gemm_tile")
 
 
 def spills(unit, log_text):
