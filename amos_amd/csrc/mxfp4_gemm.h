@@ -36,9 +36,11 @@ struct MxGemmParams {
   MxTail tail;
 };
 
+// OP: which byte of the scale registers
+template <int OP = 0>
 __device__ __forceinline__ v4f mx_mfma(mx_v4i a, mx_v4i b, v4f c, int sa, int sb) {
   const mx_v8i a8 = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, b8 = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, 0, sa, 0, sb);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a8, b8, c, 4, 4, OP, sa, OP, sb);
 }
 
 __device__ __forceinline__ float mx_tail(const MxTail& t, float v, int64_t m, int n, int N) {

@@ -145,10 +145,10 @@ static void launch_few(const MxGemmParams& p, int src, hipStream_t stream) {
 }
 
 // ---- many rows of A -----------------------------------------------------------------------------
-template <int WI, int WJ, int BI, int BJ, int NS>
+template <int WI, int WJ, int BI, int BJ>
 static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
-  constexpr int lds = NS * (BI + BJ) * 136;
-  void (*const fn)(const MxTileParams) = amos_mx_gemm_tile<WI, WJ, BI, BJ, NS>;
+  constexpr int lds = 2 * (BI + BJ) * 136;
+  void (*const fn)(const MxTileParams) = amos_mx_gemm_tile<WI, WJ, BI, BJ>;
   static std::once_flag once;
   static hipError_t err = hipSuccess;
   static int spilled = 0;
@@ -247,7 +247,7 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
   // (the tiled kernel's offsets inside a tile have 32 bits)
   if (d->M > 64 && p.steps < 1 << 18) {
     const int64_t big = ((d->M + 255) / 256) * ((d->N + 255) / 256);
-    rc = big >= 256 ? launch_tile<2, 4, 256, 256, 2>(p, stream) : launch_tile<2, 4, 128, 128, 2>(p, stream);
+    rc = big >= 256 ? launch_tile<4, 2, 256, 256>(p, stream) : launch_tile<2, 4, 128, 128>(p, stream);
     if (rc) return rc;
     const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return set_error(AMOS_ERR_HIP, "launch failed: %s", hipGetErrorString(err));

@@ -1,13 +1,14 @@
 // Tiled product of two microscaled 4-bit matrices: many rows on both sides.
 //
-// Block tile BI x BJ, K step 256 elements = 128 bytes of every row, NS stages in LDS of
-// (BI + BJ) * 136 bytes: the codes as rows of eight 16-byte chunks (XOR-swizzled by row, the swizzle
-// applied on the global side), behind them eight scale bytes a row.  Both travel by direct copies
-// (global_load_lds, 16 and 4 bytes a lane); the copies of step t + NS leave right behind the one
-// barrier of step t.  A K step is two matrix instructions deep (K = 128 each) and each of them is
-// issued in two halves over the wave tile's rows, so that the fragments of the next half are read
-// while this one multiplies.  A fragment is one 16-byte LDS read and one byte read for its block's scale: the
-// byte arrives in the register the matrix instruction takes it from, no instruction touches it.
+// Block tile BI x BJ, K step 256 elements = 128 bytes of every row, two stages in LDS of (BI + BJ) * 136
+// bytes: the codes as rows of eight 16-byte chunks (XOR-swizzled by row, the swizzle applied on the
+// global side), behind them eight scale bytes a row.  Both travel by direct copies (global_load_lds, 16
+// and 4 bytes a lane).  A K step is two matrix instructions deep and runs in four phases (half of
+// the wave tile's rows, sub-step); the fragments of a phase are read while the one before multiplies.
+// The one barrier of a step stands in front of its last phase, where all reads of the stage are
+// issued; the copies of the step after next start behind it, spread over three phases.  A fragment is
+// one 16-byte LDS read; its block's scale is a byte of a register that a 2-byte read fills for both
+// sub-steps and that the matrix instruction takes as it is: no instruction touches a scale.
 // Rows past M / N repeat the last one (their sums are not stored).  K is padded to 128 by the format; an
 // odd number of 128s ends in a half step whose second half is neither read from memory (its lanes fetch
 // the first half again: the row may be the buffer's last) nor multiplied.
@@ -35,7 +36,6 @@ __device__ __forceinline__ int mx_lds_offset(int row, int chunk) {
   return row * 128 + ((chunk ^ ((row ^ ((row >> 3) & 1)) & 7)) << 4);
 }
 
-#define AMOS_MX_GLOBAL(p) ((const __attribute__((address_space(1))) void*)(p))
 #define AMOS_MX_LDS(p) ((__attribute__((address_space(3))) void*)(p))
 
 // V consecutive values of a dense tensor; `whole`: they are aligned to V elements (or 16 bytes)
@@ -56,7 +56,7 @@ __device__ __forceinline__ void mx_load_run(const void* p, int64_t at, int dtype
   }
 }
 
-template <int WI, int WJ, int BI, int BJ, int NS>
+template <int WI, int WJ, int BI, int BJ>
 __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTileParams t) {
   constexpr int NW = WI * WJ;
   constexpr int TI = BI / (16 * WI), TJ = BJ / (16 * WJ);
@@ -66,7 +66,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   constexpr int QA = BI / 8;
   constexpr int CH = (BI + BJ) / 8 / NW, SCH = (BI + BJ) / 32 / NW;
   static_assert(CH >= 1 && CH * NW * 8 == BI + BJ && SCH >= 1 && SCH * NW * 32 == BI + BJ, "copies");
-  constexpr int COPIES = CH + SCH;
+  constexpr int COPIES = CH + SCH, NS = 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const MxGemmParams& p = t.g;
   const int lane = threadIdx.x & 63;
@@ -103,29 +103,32 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     s_off[u] = (unsigned)r * (unsigned)spitch + (lane & 1) * 4;
   }
   const unsigned back = chunk >= 4 ? 64 : 0, sback = (lane & 1) * 4;   // what a half step's second half steps back
-  auto issue_copies = [&](int kt, int stage) {
+  // Copy u of step kt (the codes first, then the scales).  As assembly: behind the builtin the compiler lets every
+  // later LDS read wait for all LDS reads before it.  The wait states are those of an address register pair that
+  // a vector instruction may have written (5) and of M0 (1).
+  const unsigned lds0 = (unsigned)(uintptr_t)AMOS_MX_LDS(smem);
+  auto issue_copy = [&](int kt, int stage, int u) {
     const bool h = kt >= full;
-    const unsigned char *ak = abase + (int64_t)kt * 128 - (h ? back : 0u), *bk = bbase + (int64_t)kt * 128 - (h ? back : 0u);
-    const unsigned char *as = asbase + (int64_t)kt * 8 - (h ? sback : 0u), *bs = bsbase + (int64_t)kt * 8 - (h ? sback : 0u);
-    char* s = smem + stage * STAGE;
-#pragma unroll
-    for (int u = 0; u < CH; ++u) {
+    const unsigned s = lds0 + stage * STAGE;
+    if (u < CH) {
       const int q = wave + NW * u;
-      __builtin_amdgcn_global_load_lds(AMOS_MX_GLOBAL((q < QA ? ak : bk) + g_off[u]), AMOS_MX_LDS(s + q * 1024), 16, 0, 0);
-    }
-#pragma unroll
-    for (int u = 0; u < SCH; ++u) {
-      const int q = wave + NW * u;
-      __builtin_amdgcn_global_load_lds(AMOS_MX_GLOBAL((q * 32 < BI ? as : bs) + s_off[u]), AMOS_MX_LDS(s + CODES + q * 256), 4, 0, 0);
+      const unsigned char* const base = (q < QA ? abase : bbase) + (int64_t)kt * 128;
+      const unsigned off = g_off[u] - (h ? back : 0u);
+      asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(s + q * 1024), "v"(off), "s"(base) : "memory");
+    } else {
+      const int q = wave + NW * (u - CH);
+      const unsigned char* const base = (q * 32 < BI ? asbase : bsbase) + (int64_t)kt * 8;
+      const unsigned off = s_off[u - CH] - (h ? sback : 0u);
+      asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(s + CODES + q * 256), "v"(off), "s"(base) : "memory");
     }
   };
 
-  // which of a sub-step's four blocks a lane group takes is free as long as both operands agree; groups q and
-  // q + 2 take neighbouring chunks, which the swizzle puts on different banks
+  // Which of a K step's eight blocks a lane group takes is free as long as both operands agree: group q takes blocks
+  // 2q and 2q + 1, whose scales are the two bytes of one read.  (A half step has four blocks: block q.)
   const int frag_row = lane & 15, frag_q = lane >> 4;
-  const int frag_chunk = (frag_q >> 1) | ((frag_q & 1) << 1);
-  const int a_off = mx_lds_offset(wi * TI * 16 + frag_row, frag_chunk), b_off = OPER + mx_lds_offset(wj * TJ * 16 + frag_row, frag_chunk);
-  const int as_off = CODES + (wi * TI * 16 + frag_row) * 8 + frag_chunk, bs_off = CODES + (BI + wj * TJ * 16 + frag_row) * 8 + frag_chunk;
+  const int arow = wi * TI * 16 + frag_row, brow = wj * TJ * 16 + frag_row;
+  const int a_off = mx_lds_offset(arow, 2 * frag_q), b_off = OPER + mx_lds_offset(brow, 2 * frag_q);
+  const int as_off = CODES + arow * 8 + 2 * frag_q, bs_off = CODES + (BI + brow) * 8 + 2 * frag_q;
 
   v4f acc[TI][TJ];
 #pragma unroll
@@ -133,62 +136,93 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
 #pragma unroll
     for (int b = 0; b < TJ; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  mx_v4i af[2][HA], bf[2][TJ];
-  int ax[2][HA], bx[2][TJ];
-  auto read_a = [&](int stage, int ks, int h, int slot) {
+  mx_v4i af[2][HA], bf[2][TJ];      // A: by half of the wave tile's rows; B: by sub-step
+  int ax[TI], bx[TJ], bx_next[TJ];   // scales: a register serves both sub-steps
+  auto read_a = [&](int stage, auto h, auto ks) {
     const char* s = smem + stage * STAGE;
 #pragma unroll
     for (int a = 0; a < HA; ++a) {
-      const int ab = h * HA + a;
-      af[slot][a] = *(const mx_v4i*)(s + (a_off ^ (ks * 64)) + ab * 2048);
-      ax[slot][a] = *(const unsigned char*)(s + as_off + ab * 128 + ks * 4);
+      af[h][a] = *(const mx_v4i*)(s + (a_off ^ (ks * 16)) + (h * HA + a) * 2048);
+      if (ks == 0) ax[h * HA + a] = *(const unsigned short*)(s + as_off + (h * HA + a) * 128);
     }
   };
-  auto read_b = [&](int stage, int ks, int slot) {
+  auto read_b = [&](int stage, auto ks, int* x) {
     const char* s = smem + stage * STAGE;
 #pragma unroll
     for (int b = 0; b < TJ; ++b) {
-      bf[slot][b] = *(const mx_v4i*)(s + (b_off ^ (ks * 64)) + b * 2048);
-      bx[slot][b] = *(const unsigned char*)(s + bs_off + b * 128 + ks * 4);
+      bf[ks][b] = *(const mx_v4i*)(s + (b_off ^ (ks * 16)) + b * 2048);
+      if (ks == 0) x[b] = *(const unsigned short*)(s + bs_off + b * 128);
     }
   };
-  auto mma = [&](int h, int sa, int sb) {
+  // One phase: the matrix instructions of half h of sub-step ks, and between them a share of the copies of step kt (a
+  // copy keeps its wave from issuing for some 64 cycles: spread out, the matrix core works through them).  The fences
+  // keep the compiler from moving the reads in front of a phase down to their use.
+  constexpr int PERG = (COPIES + 3 * TJ - 1) / (3 * TJ);   // copies behind a group of HA instructions: three phases carry them
+  auto phase = [&](auto h, auto ks, int part, int kt, int stage) {
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int b = 0; b < TJ; ++b)
+    for (int b = 0; b < TJ; ++b) {
 #pragma unroll
-      for (int a = 0; a < HA; ++a) acc[h * HA + a][b] = mx_mfma(af[sa][a], bf[sb][b], acc[h * HA + a][b], ax[sa][a], bx[sb][b]);
+      for (int a = 0; a < HA; ++a) acc[h * HA + a][b] = mx_mfma<ks>(af[h][a], bf[ks][b], acc[h * HA + a][b], ax[h * HA + a], bx[b]);
+      if (part >= 0) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < PERG; ++i) {
+          const int u = (part * TJ + b) * PERG + i;
+          if (u < COPIES) issue_copy(kt, stage, u);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
   };
+  constexpr std::integral_constant<int, 0> I0{};
+  constexpr std::integral_constant<int, 1> I1{};
+  constexpr int FIRST = PERG * TJ < COPIES ? PERG * TJ : COPIES;   // copies of part 0
 
-  static_assert(NS >= 2 && (NS - 1) * COPIES <= 63, "stages");
+  // step 0 whole, of step 1 the part that otherwise leaves in the step before
 #pragma unroll
-  for (int s = 0; s < NS; ++s) issue_copies(s < KT ? s : KT - 1, s);
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * COPIES) : "memory");
-  read_a(0, 0, 0, 0);
-  read_b(0, 0, 0);
+  for (int u = 0; u < COPIES; ++u) issue_copy(0, 0, u);
+#pragma unroll
+  for (int u = 0; u < FIRST; ++u) issue_copy(1 < KT ? 1 : KT - 1, 1, u);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(FIRST) : "memory");
+  read_a(0, I0, I0);
+  read_b(0, I0, bx);
 
-  int st = 0;
   for (int kt = 0; kt < full; ++kt) {
-    const int st_next = st + 1 == NS ? 0 : st + 1;
-    read_a(st, 0, 1, 1);
-    mma(0, 0, 0);
-    read_a(st, 1, 0, 0);
-    read_b(st, 1, 1);
-    mma(1, 1, 0);
-    read_a(st, 1, 1, 1);
-    mma(0, 0, 1);
-    // all reads of this stage are issued; once they and this wave's copies of the next tile are done, meet: behind
-    // the barrier the next stage is whole and this one is free
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((NS - 2) * COPIES) : "memory");
-    issue_copies(kt + NS < KT ? kt + NS : KT - 1, st);
-    read_a(st_next, 0, 0, 0);   // (behind the last step: read and not used)
-    read_b(st_next, 0, 0);
-    mma(1, 1, 1);
-    st = st_next;
+    const int st = kt & 1, next = kt + 1 < KT ? kt + 1 : KT - 1, after = kt + 2 < KT ? kt + 2 : KT - 1;
+    read_a(st, I1, I0);
+    phase(I0, I0, 1, next, st ^ 1);
+    read_a(st, I0, I1);
+    read_b(st, I1, bx);
+    phase(I1, I0, 2, next, st ^ 1);
+    read_a(st, I1, I1);
+    phase(I0, I1, -1, 0, 0);
+    // all reads of this stage are issued; once they and this wave's copies of the next step are done, meet: behind the
+    // barrier the next stage is whole and this one is free
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    read_a(st ^ 1, I0, I0);   // (behind the last step: read and not used)
+    read_b(st ^ 1, I0, bx_next);
+    phase(I1, I1, 0, after, st);
+#pragma unroll
+    for (int b = 0; b < TJ; ++b) bx[b] = bx_next[b];
   }
-  if (half) {
-    read_a(st, 0, 1, 1);
-    mma(0, 0, 0);
-    mma(1, 1, 0);
+  if (half) {   // four blocks, one for each lane group
+    const char* s = smem + (full & 1) * STAGE;
+    const int ah = mx_lds_offset(arow, frag_q), bh = OPER + mx_lds_offset(brow, frag_q);
+    const int axh = CODES + arow * 8 + frag_q, bxh = CODES + (BI + brow) * 8 + frag_q;
+#pragma unroll
+    for (int b = 0; b < TJ; ++b) {
+      bf[0][b] = *(const mx_v4i*)(s + bh + b * 2048);
+      bx[b] = *(const unsigned char*)(s + bxh + b * 128);
+    }
+#pragma unroll
+    for (int a = 0; a < TI; ++a) {
+      const mx_v4i f = *(const mx_v4i*)(s + ah + a * 2048);
+      const int x = *(const unsigned char*)(s + axh + a * 128);
+#pragma unroll
+      for (int b = 0; b < TJ; ++b) acc[a][b] = mx_mfma(f, bf[0][b], acc[a][b], x, bx[b]);
+    }
   }
 
   // ---- the sums leave through a strip of LDS per wave (half the wave tile's rows at a time): whole rows, 16 bytes
