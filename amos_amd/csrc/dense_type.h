@@ -38,11 +38,12 @@ template <class T, int N>
 struct DenseVec {
   typedef typename T::raw_t raw_t;
   typedef raw_t vec_t __attribute__((ext_vector_type(N)));
-  static __device__ __forceinline__ void load(const raw_t* p, float* v) {
-    const vec_t x = *(const vec_t*)p;
+  static __device__ __forceinline__ vec_t read(const raw_t* p) { return *(const vec_t*)p; }
+  static __device__ __forceinline__ void widen(vec_t x, float* v) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = T::widen(x[i]);
   }
+  static __device__ __forceinline__ void load(const raw_t* p, float* v) { widen(read(p), v); }
   static __device__ __forceinline__ void store(raw_t* p, const float* v) {
     vec_t x;
 #pragma unroll
@@ -56,6 +57,31 @@ __device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
   if (dtype == AMOS_F32) return ((const float*)p)[i];
   if (dtype == AMOS_F16) return TypeF16::widen(((const _Float16*)p)[i]);
   return TypeBF16::widen(((const __bf16*)p)[i]);
+}
+// N of them in a row, or `otherwise` where there is no tensor: the type is looked at once, the loads
+// are in flight together
+template <int N>
+__device__ __forceinline__ void load_run_any(const void* p, int64_t at, int dtype, float otherwise, float* v) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = otherwise;
+  } else if (dtype == AMOS_F32) {
+    const float* const q = (const float*)p + at;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = q[i];
+  } else {
+    const unsigned short* const q = (const unsigned short*)p + at;
+    unsigned short raw[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) raw[i] = q[i];
+    if (dtype == AMOS_F16) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = TypeF16::widen(__builtin_bit_cast(_Float16, raw[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = TypeBF16::widen(__builtin_bit_cast(__bf16, raw[i]));
+    }
+  }
 }
 __device__ __forceinline__ void store_any(void* p, int64_t i, int dtype, float v) {
   if (dtype == AMOS_F32) ((float*)p)[i] = v;

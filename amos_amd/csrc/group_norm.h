@@ -43,6 +43,8 @@ struct GnParams {
   float eps;
   int act, affine_dtype;
   FastDiv by_cpg, by_cols;
+  FastDiv by_epg;            // one-launch kernels: entries of a group in a row of threads
+  int y_dtype;
 };
 
 // sums over the pixels of one group are kept as (count, mean, sum of squared deviations): no
@@ -115,7 +117,76 @@ __device__ __forceinline__ float gn_team_sum(float v, int team) {
 
 struct GnPlan {
   int vec;
+  bool uni;                  // a vector lies inside one group
+  int held;                  // pixels a thread of the one-launch kernel holds (0: two launches)
+  int threads, lds;          // of that kernel
   int64_t part_floats, cpart_floats;
 };
+
+// ---- the one-launch kernels: a slab of whole groups of one image is held in registers -------------
+// A workgroup takes p.ct channels (whole groups) of one image; a lane keeps VEC channels of the pixels row,
+// row + rows, ...  UNI: a vector lies inside one group.
+struct GnSlab {
+  int n, c0, g0, groups;
+  int col, row, c;               // of this thread; its first channel
+  bool active;
+};
+__device__ __forceinline__ GnSlab gn_slab(const GnParams& p, int vec) {
+  GnSlab w;
+  int b = blockIdx.x, slab;
+  // slabs of an image share memory lines: where images come in eights, an image's slabs go to one XCD
+  // (workgroups are dealt to the eight in launch order)
+  if ((p.N & 7) == 0) {
+    const int s = b >> 3, image = s / p.tiles;
+    w.n = (b & 7) + 8 * image;
+    slab = s - image * p.tiles;
+  } else {
+    w.n = b / p.tiles;
+    slab = b - w.n * p.tiles;
+  }
+  w.c0 = slab * p.ct;
+  w.g0 = w.c0 / p.cpg;
+  w.groups = p.ct / p.cpg;
+  const int t = threadIdx.x;
+  w.row = fast_div(t, p.by_cols);
+  w.col = t - w.row * p.cols;
+  w.active = w.row < p.rows;
+  w.c = w.c0 + w.col * vec;
+  return w;
+}
+// Sums over each group of a slab: the threads' values `v` (one each for UNI, else one for each channel) meet in
+// `lds` ([rows][entries]), a team of lanes adds a group's, in an order that does not depend on timing; totals in
+// `total` [groups].  Barriers in front, between and behind.
+template <int VEC, bool UNI>
+__device__ __forceinline__ void gn_group_sums(const GnParams& p, const GnSlab& w, const float* v, float* lds, float* total) {
+  const int per = UNI ? p.cols : p.cols * VEC;
+  const int epg = per / w.groups;
+  if (w.active) {
+    if (UNI) lds[w.row * per + w.col] = v[0];
+    else
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) lds[w.row * per + w.col * VEC + i] = v[i];
+  }
+  __syncthreads();
+  int team = 64;
+  while (team > 1 && team * w.groups > (int)blockDim.x) team >>= 1;
+  const int lane = threadIdx.x & (team - 1), step = (int)blockDim.x / team, entries = p.rows * epg;
+  for (int g = threadIdx.x / team; g < w.groups; g += step) {
+    float s = 0.f;
+    for (int e = lane; e < entries; e += team) {
+      const int r = fast_div(e, p.by_epg);
+      s += lds[r * per + g * epg + (e - r * epg)];
+    }
+    s = gn_team_sum(s, team);
+    if (lane == 0) total[g] = s;
+  }
+  __syncthreads();
+}
+template <int VEC>
+__device__ __forceinline__ void gn_store_any(void* p, int64_t at, int dtype, const float* v) {
+  if (dtype == AMOS_F32) DenseVec<TypeF32, VEC>::store((float*)p + at, v);
+  else if (dtype == AMOS_F16) DenseVec<TypeF16, VEC>::store((_Float16*)p + at, v);
+  else DenseVec<TypeBF16, VEC>::store((__bf16*)p + at, v);
+}
 
 }  // namespace amos

@@ -1,3 +1,5 @@
+#include <mutex>
+
 #include "group_norm.h"
 #include "group_norm_host.h"
 
@@ -14,9 +16,9 @@ struct GnChannels {
       const int64_t g = (int64_t)n * p.G + fast_div(c, p.by_cpg);
       mean[i] = p.mean[g];
       rstd[i] = p.rstd[g];
-      weight[i] = p.weight ? load_any(p.weight, c, p.affine_dtype) : 1.f;
-      bias[i] = p.bias ? load_any(p.bias, c, p.affine_dtype) : 0.f;
     }
+    load_run_any<VEC>(p.weight, c0, p.affine_dtype, 1.f, weight);
+    load_run_any<VEC>(p.bias, c0, p.affine_dtype, 0.f, bias);
   }
 };
 
@@ -33,16 +35,29 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_partial(const GnP
     float a1[VEC], a2[VEC];
 #pragma unroll
     for (int i = 0; i < VEC; ++i) a1[i] = a2[i] = 0.f;
-    for (int q = w.p0 + w.row; q < w.p1; q += p.rows) {
-      float v[VEC], g[VEC];
-      DenseVec<XT, VEC>::load(x + (int64_t)q * p.pixel, v);
-      DenseVec<YT, VEC>::load(dy + (int64_t)q * p.pixel, g);
+    constexpr int B = VEC * XT::ES > 16 || VEC * YT::ES > 16 ? 2 : 4;   // pixels in flight
+    for (int q = w.p0 + w.row; q < w.p1; q += B * p.rows) {
+      typename DenseVec<XT, VEC>::vec_t rx[B];
+      typename DenseVec<YT, VEC>::vec_t rg[B];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) {
-        const float h = (v[i] - ch.mean[i]) * ch.rstd[i];
-        const float d = gn_act_gradient(g[i], h * ch.weight[i] + ch.bias[i], p.act);
-        a1[i] += d;
-        a2[i] += d * h;
+      for (int u = 0; u < B; ++u) {   // (past the end: the last pixel again, left out of the sums)
+        const int at = q + u * p.rows < w.p1 ? q + u * p.rows : w.p1 - 1;
+        rx[u] = DenseVec<XT, VEC>::read(x + (int64_t)at * p.pixel);
+        rg[u] = DenseVec<YT, VEC>::read(dy + (int64_t)at * p.pixel);
+      }
+#pragma unroll
+      for (int u = 0; u < B; ++u) {
+        if (q + u * p.rows >= w.p1) break;
+        float v[VEC], g[VEC];
+        DenseVec<XT, VEC>::widen(rx[u], v);
+        DenseVec<YT, VEC>::widen(rg[u], g);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float h = (v[i] - ch.mean[i]) * ch.rstd[i];
+          const float d = gn_act_gradient(g[i], h * ch.weight[i] + ch.bias[i], p.act);
+          a1[i] += d;
+          a2[i] += d * h;
+        }
       }
     }
 #pragma unroll
@@ -88,7 +103,7 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_partial(const GnP
 // dweight, dbias: sixteen channels a workgroup, sixteen rows of partial sums side by side
 __device__ __forceinline__ void gn_coefficient_gradients(const GnParams& p, int block, float* s1, float* s2) {
   const int t = threadIdx.x, c = block * 16 + (t & 15), r0 = t >> 4;
-  const int rows = p.N * p.chunks;
+  const int rows = p.N * p.chunks;   // (one-launch kernel: a row an image)
   float a = 0.f, b = 0.f;
   if (c < p.C) {
     const float* at = p.cpart + (int64_t)c * 2;
@@ -120,6 +135,7 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_apply(const GnPar
     return;
   }
   const GnTile w = gn_tile<VEC>(p, blockIdx.x);
+  const GnChannels<VEC> ch(p, w.n, w.c0 + (w.active ? w.col * VEC : 0));
   {
     const int team = gn_team(w.groups), t = threadIdx.x, lane = t & (team - 1);
     const float share = 1.f / ((float)p.P * p.cpg);
@@ -140,7 +156,6 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_apply(const GnPar
   }
   __syncthreads();
   if (!w.active) return;
-  const GnChannels<VEC> ch(p, w.n, w.c0 + w.col * VEC);
   float e1[VEC], e2[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
@@ -152,18 +167,194 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_apply(const GnPar
   const typename XT::raw_t* const x = (const typename XT::raw_t*)p.x + base;
   const typename YT::raw_t* const dy = (const typename YT::raw_t*)p.dy + base;
   typename XT::raw_t* const dx = (typename XT::raw_t*)p.out + base;
-  for (int q = w.p0 + w.row; q < w.p1; q += p.rows) {
+  constexpr int B = VEC * XT::ES > 16 || VEC * YT::ES > 16 ? 2 : 4;   // pixels in flight
+  for (int q = w.p0 + w.row; q < w.p1; q += B * p.rows) {
+    typename DenseVec<XT, VEC>::vec_t rx[B];
+    typename DenseVec<YT, VEC>::vec_t rg[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      const int at = q + u * p.rows < w.p1 ? q + u * p.rows : w.p1 - 1;
+      rx[u] = DenseVec<XT, VEC>::read(x + (int64_t)at * p.pixel);
+      rg[u] = DenseVec<YT, VEC>::read(dy + (int64_t)at * p.pixel);
+    }
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      if (q + u * p.rows >= w.p1) break;
+      float v[VEC], g[VEC];
+      DenseVec<XT, VEC>::widen(rx[u], v);
+      DenseVec<YT, VEC>::widen(rg[u], g);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float h = (v[i] - ch.mean[i]) * ch.rstd[i];
+        const float d = gn_act_gradient(g[i], h * ch.weight[i] + ch.bias[i], p.act);
+        v[i] = (d * ch.weight[i] - e1[i] - h * e2[i]) * ch.rstd[i];
+      }
+      DenseVec<XT, VEC>::store(dx + (int64_t)(q + u * p.rows) * p.pixel, v);
+    }
+  }
+}
+
+// ---- one launch: x and dy of a slab of whole groups stay in registers between the sums and dx -----------
+template <class XT, class YT, int VEC, int R>
+__global__ __launch_bounds__(1024) void amos_gn_gradient_held(const GnParams p) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  typedef DenseVec<XT, VEC> VX;
+  typedef DenseVec<YT, VEC> VY;
+  const GnSlab w = gn_slab(p, VEC);
+  const int T = (int)blockDim.x, t = threadIdx.x;
+  float *const s1 = lds, *const s2 = lds + p.rows * p.ct, *const e1 = lds + 2 * p.rows * p.ct, *const e2 = e1 + w.groups;
+  const int64_t base = w.n * p.image + w.c;
+  typename VX::vec_t rx[R];
+  typename VY::vec_t rg[R];
+  const int c0 = w.active ? w.c : w.c0;
+  if (w.active) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {   // (pixels past the end: the last one again, left out of the sums)
+      const int q = w.row + r * p.rows < p.P ? w.row + r * p.rows : p.P - 1;
+      rx[r] = VX::read((const typename XT::raw_t*)p.x + base + (int64_t)q * p.pixel);
+      rg[r] = VY::read((const typename YT::raw_t*)p.dy + base + (int64_t)q * p.pixel);
+    }
+  }
+  const GnChannels<VEC> ch(p, w.n, c0);
+  if (w.active) {
+    float a1[VEC], a2[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) a1[i] = a2[i] = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (w.row + r * p.rows >= p.P) break;
+      float v[VEC], g[VEC];
+      VX::widen(rx[r], v);
+      VY::widen(rg[r], g);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const float h = (v[i] - ch.mean[i]) * ch.rstd[i];
+        const float d = gn_act_gradient(g[i], h * ch.weight[i] + ch.bias[i], p.act);
+        a1[i] += d;
+        a2[i] += d * h;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      s1[w.row * p.ct + w.col * VEC + i] = a1[i];
+      s2[w.row * p.ct + w.col * VEC + i] = a2[i];
+    }
+  }
+  __syncthreads();
+  // ---- the pixel rows meet: up to `parts` threads a channel, then one
+  int parts = T / p.ct < 32 ? T / p.ct : 32;
+  if (parts > p.rows) parts = p.rows;
+  if (parts > 1) {
+    const int c = t % p.ct, part = t / p.ct;
+    float a = 0.f, b = 0.f;
+    if (part < parts) {
+      for (int r = part; r < p.rows; r += parts) {
+        a += s1[r * p.ct + c];
+        b += s2[r * p.ct + c];
+      }
+      s1[part * p.ct + c] = a;   // (row `part`: read by this thread only)
+      s2[part * p.ct + c] = b;
+    }
+    __syncthreads();
+  } else {
+    parts = p.rows;
+  }
+  for (int c = t; c < p.ct; c += T) {
+    float a = 0.f, b = 0.f;
+    for (int r = 0; r < parts; ++r) {
+      a += s1[r * p.ct + c];
+      b += s2[r * p.ct + c];
+    }
+    const int at = w.c0 + c;
+    if (p.N == 1) {
+      if (p.dbias) p.dbias[at] = a;
+      if (p.dweight) p.dweight[at] = b;
+    } else if (p.dbias || p.dweight) {
+      float* const cp = p.cpart + ((int64_t)w.n * p.C + at) * 2;
+      cp[0] = a;
+      cp[1] = b;
+    }
+    const float weight = p.weight ? load_any(p.weight, at, p.affine_dtype) : 1.f;
+    s1[c] = a * weight;
+    s2[c] = b * weight;
+  }
+  __syncthreads();
+  {
+    int team = 64;
+    while (team > 1 && team * w.groups > T) team >>= 1;
+    const int lane = t & (team - 1);
+    const float count = (float)p.P * p.cpg;
+    for (int g = t / team; g < w.groups; g += T / team) {
+      float a = 0.f, b = 0.f;
+      for (int e = lane; e < p.cpg; e += team) {
+        a += s1[g * p.cpg + e];
+        b += s2[g * p.cpg + e];
+      }
+      a = gn_team_sum(a, team);
+      b = gn_team_sum(b, team);
+      if (lane == 0) {
+        e1[g] = a / count;
+        e2[g] = b / count;
+      }
+    }
+  }
+  __syncthreads();
+  if (!w.active) return;
+  float m1[VEC], m2[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    const int g = fast_div(w.c + i, p.by_cpg) - w.g0;
+    m1[i] = e1[g];
+    m2[i] = e2[g];
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int q = w.row + r * p.rows;
+    if (q >= p.P) break;
     float v[VEC], g[VEC];
-    DenseVec<XT, VEC>::load(x + (int64_t)q * p.pixel, v);
-    DenseVec<YT, VEC>::load(dy + (int64_t)q * p.pixel, g);
+    VX::widen(rx[r], v);
+    VY::widen(rg[r], g);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       const float h = (v[i] - ch.mean[i]) * ch.rstd[i];
       const float d = gn_act_gradient(g[i], h * ch.weight[i] + ch.bias[i], p.act);
-      v[i] = (d * ch.weight[i] - e1[i] - h * e2[i]) * ch.rstd[i];
+      v[i] = (d * ch.weight[i] - m1[i] - h * m2[i]) * ch.rstd[i];
     }
-    DenseVec<XT, VEC>::store(dx + (int64_t)q * p.pixel, v);
+    VX::store((typename XT::raw_t*)p.out + base + (int64_t)q * p.pixel, v);
   }
+}
+
+// dweight and dbias from the images' shares
+__global__ __launch_bounds__(kGnThreads) void amos_gn_coefficients(const GnParams p) {
+  __shared__ float s1[kGnThreads], s2[kGnThreads];
+  gn_coefficient_gradients(p, (int)blockIdx.x, s1, s2);
+}
+
+template <class XT, class YT, int VEC, int R>
+static int launch_held(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
+  void (*const fn)(const GnParams) = amos_gn_gradient_held<XT, YT, VEC, R>;
+  static std::once_flag once;
+  static hipError_t err = hipSuccess;
+  std::call_once(once, [&] { err = hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024); });
+  if (err != hipSuccess) return set_error(AMOS_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(err));
+  hipLaunchKernelGGL(fn, dim3((unsigned)((int64_t)p.N * p.tiles)), dim3((unsigned)plan.threads), plan.lds, stream, p);
+  if (p.N > 1 && (p.dweight || p.dbias)) hipLaunchKernelGGL(amos_gn_coefficients, dim3((unsigned)((p.C + 15) / 16)), dim3(kGnThreads), 0, stream, p);
+  return 0;
+}
+template <class XT, class YT, int VEC>
+static int launch_held_by(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
+  if (plan.held <= 2) return launch_held<XT, YT, VEC, 2>(p, plan, stream);
+  return launch_held<XT, YT, VEC, kGnHeldGradient>(p, plan, stream);
+}
+template <class XT, class YT>
+static int pick_held(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
+  if constexpr (XT::ES == 2 && YT::ES == 2) {
+    if (plan.vec == 8) return launch_held_by<XT, YT, 8>(p, plan, stream);
+  }
+  if constexpr (XT::ES == 4 || YT::ES == 4) {
+    if (plan.vec == 4) return launch_held_by<XT, YT, 4>(p, plan, stream);
+  }
+  return launch_held_by<XT, YT, 1>(p, plan, stream);
 }
 
 template <class XT, class YT, int VEC>
@@ -174,25 +365,30 @@ static void launch(const GnParams& p, hipStream_t stream) {
   hipLaunchKernelGGL((amos_gn_gradient_apply<XT, YT, VEC>), dim3(work + more, (unsigned)p.tiles), dim3(kGnThreads), 0, stream, p);
 }
 template <class XT, class YT>
-static void pick_vec(const GnParams& p, int vec, hipStream_t stream) {
-  if (vec == 8) launch<XT, YT, 8>(p, stream);
+static int pick_kernel(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
+  if (plan.held) return pick_held<XT, YT>(p, plan, stream);
+  constexpr int WIDE = XT::ES == 4 || YT::ES == 4 ? 4 : 8;   // 16 bytes of the wider type
+  if (plan.vec == WIDE) launch<XT, YT, WIDE>(p, stream);
   else launch<XT, YT, 1>(p, stream);
+  return 0;
 }
 template <class XT>
-static void pick_out(const GnParams& p, int vec, int y_dtype, hipStream_t stream) {
-  if (y_dtype == AMOS_F32) pick_vec<XT, TypeF32>(p, vec, stream);
-  else if (y_dtype == AMOS_F16) pick_vec<XT, TypeF16>(p, vec, stream);
-  else pick_vec<XT, TypeBF16>(p, vec, stream);
+static int pick_out(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
+  if (p.y_dtype == AMOS_F32) return pick_kernel<XT, TypeF32>(p, plan, stream);
+  if (p.y_dtype == AMOS_F16) return pick_kernel<XT, TypeF16>(p, plan, stream);
+  return pick_kernel<XT, TypeBF16>(p, plan, stream);
 }
 
 static int run_gradient(const amos_group_norm_desc_t* d, const void* dy, const void* x, const void* weight, const void* bias, const float* mean,
                         const float* rstd, void* dx, float* dweight, float* dbias, void* workspace, size_t ws_bytes, hipStream_t stream) {
   GnParams p;
   GnPlan plan;
-  int rc = gn_plan(d, {dy, x, dx}, weight, bias, p, plan);
+  bool wide;
+  int rc = gn_check(d, {dy, x, dx}, weight, bias, p, wide);
   if (rc) return rc;
   if (!mean || !rstd) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
-  rc = gn_workspace(plan, p, true, workspace, ws_bytes);
+  rc = gn_choose(d, true, wide, p, plan);
+  if (rc == 0) rc = gn_workspace(plan, p, workspace, ws_bytes);
   if (rc) return rc;
   p.x = x;
   p.dy = dy;
@@ -201,9 +397,10 @@ static int run_gradient(const amos_group_norm_desc_t* d, const void* dy, const v
   p.rstd = (float*)rstd;
   p.dweight = dweight;
   p.dbias = dbias;
-  if (d->x_dtype == AMOS_F32) pick_out<TypeF32>(p, plan.vec, d->y_dtype, stream);
-  else if (d->x_dtype == AMOS_F16) pick_out<TypeF16>(p, plan.vec, d->y_dtype, stream);
-  else pick_out<TypeBF16>(p, plan.vec, d->y_dtype, stream);
+  if (d->x_dtype == AMOS_F32) rc = pick_out<TypeF32>(p, plan, stream);
+  else if (d->x_dtype == AMOS_F16) rc = pick_out<TypeF16>(p, plan, stream);
+  else rc = pick_out<TypeBF16>(p, plan, stream);
+  if (rc) return rc;
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(AMOS_ERR_HIP, "launch failed: %s", hipGetErrorString(e));
   return 0;

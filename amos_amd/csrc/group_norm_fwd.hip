@@ -109,6 +109,9 @@ template <class XT, class YT, int VEC>
 __global__ __launch_bounds__(kGnThreads) void amos_gn_apply(const GnParams p) {
   __shared__ float smean[kGnThreads * VEC], srstd[kGnThreads * VEC];   // by group of the tile
   const GnTile w = gn_tile<VEC>(p, blockIdx.x);
+  float m[VEC], a[VEC], b[VEC];
+  load_run_any<VEC>(p.weight, w.c0 + (w.active ? w.col * VEC : 0), p.affine_dtype, 1.f, a);
+  load_run_any<VEC>(p.bias, w.c0 + (w.active ? w.col * VEC : 0), p.affine_dtype, 0.f, b);
   {
     const int team = gn_team(w.groups), t = threadIdx.x, lane = t & (team - 1), step = kGnThreads / team;
     for (int g = t / team; g < w.groups; g += step) {
@@ -126,25 +129,141 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_apply(const GnParams p) {
   }
   __syncthreads();
   if (!w.active) return;
-  float m[VEC], a[VEC], b[VEC];
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    const int c = w.c0 + w.col * VEC + i;
-    const int g = fast_div(c, p.by_cpg) - w.g0;
+    const int g = fast_div(w.c0 + w.col * VEC + i, p.by_cpg) - w.g0;
     m[i] = smean[g];
-    a[i] = srstd[g] * (p.weight ? load_any(p.weight, c, p.affine_dtype) : 1.f);
-    b[i] = p.bias ? load_any(p.bias, c, p.affine_dtype) : 0.f;
+    a[i] *= srstd[g];
   }
   const int64_t base = w.n * p.image + w.c0 + w.col * VEC;
   const typename XT::raw_t* const x = (const typename XT::raw_t*)p.x + base;
   typename YT::raw_t* const y = (typename YT::raw_t*)p.out + base;
-  for (int q = w.p0 + w.row; q < w.p1; q += p.rows) {
+  constexpr int B = 4;
+  int q = w.p0 + w.row;
+  for (; q + (B - 1) * p.rows < w.p1; q += B * p.rows) {   // four pixels in flight
+    typename DenseVec<XT, VEC>::vec_t raw[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) raw[u] = DenseVec<XT, VEC>::read(x + (int64_t)(q + u * p.rows) * p.pixel);
+#pragma unroll
+    for (int u = 0; u < B; ++u) {
+      float v[VEC];
+      DenseVec<XT, VEC>::widen(raw[u], v);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) v[i] = gn_act((v[i] - m[i]) * a[i] + b[i], p.act);
+      DenseVec<YT, VEC>::store(y + (int64_t)(q + u * p.rows) * p.pixel, v);
+    }
+  }
+  for (; q < w.p1; q += p.rows) {
     float v[VEC];
     DenseVec<XT, VEC>::load(x + (int64_t)q * p.pixel, v);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[i] = gn_act((v[i] - m[i]) * a[i] + b[i], p.act);
     DenseVec<YT, VEC>::store(y + (int64_t)q * p.pixel, v);
   }
+}
+
+// ---- one launch: a slab of whole groups stays in registers between the sums and the output -----------
+// One pass over memory.  A thread holds R vectors of 16 bytes (all its loads are in flight together); mean, then the
+// squared deviations from it, from the registers.
+template <class XT, int VEC, int R, bool UNI>
+__global__ __launch_bounds__(1024) void amos_gn_held(const GnParams p) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  typedef DenseVec<XT, VEC> V;
+  const GnSlab w = gn_slab(p, VEC);
+  const int per = UNI ? p.cols : p.cols * VEC;
+  float* const total = lds + p.rows * per;
+  const typename XT::raw_t* const x = (const typename XT::raw_t*)p.x + w.n * p.image + w.c;
+  typename V::vec_t raw[R];
+  if (w.active) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {   // (pixels past the end: the last one again, left out of the sums)
+      const int q = w.row + r * p.rows;
+      raw[r] = V::read(x + (int64_t)(q < p.P ? q : p.P - 1) * p.pixel);
+    }
+  }
+  float gamma[VEC], beta[VEC];
+  load_run_any<VEC>(p.weight, w.active ? w.c : w.c0, p.affine_dtype, 1.f, gamma);
+  load_run_any<VEC>(p.bias, w.active ? w.c : w.c0, p.affine_dtype, 0.f, beta);
+  constexpr int S = UNI ? 1 : VEC;   // sums a thread keeps
+  float s[S], mean[S], rstd[S];
+  int group[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) group[i] = w.active ? fast_div(w.c + i, p.by_cpg) - w.g0 : 0;
+  const float count = (float)p.P * p.cpg;   // (divided by, not multiplied with its inverse: equal values have their own mean)
+#pragma unroll
+  for (int i = 0; i < S; ++i) s[i] = 0.f;
+  if (w.active) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float v[VEC];
+      V::widen(raw[r], v);
+      if (w.row + r * p.rows < p.P) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[UNI ? 0 : i] += v[i];
+      }
+    }
+  }
+  gn_group_sums<VEC, UNI>(p, w, s, lds, total);
+#pragma unroll
+  for (int i = 0; i < S; ++i) {
+    mean[i] = total[group[i]] / count;
+    s[i] = 0.f;
+  }
+  if (w.active) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float v[VEC];
+      V::widen(raw[r], v);
+      if (w.row + r * p.rows < p.P) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          const float d = v[i] - mean[UNI ? 0 : i];
+          s[UNI ? 0 : i] += d * d;
+        }
+      }
+    }
+  }
+  gn_group_sums<VEC, UNI>(p, w, s, lds, total + w.groups);
+#pragma unroll
+  for (int i = 0; i < S; ++i) rstd[i] = 1.f / sqrtf(total[w.groups + group[i]] / count + p.eps);
+  if (!w.active) return;
+  if (w.row == 0) {   // a group's first lane and channel
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      if ((w.g0 + group[i]) * p.cpg == w.c + i) {
+        if (p.mean) p.mean[(int64_t)w.n * p.G + w.g0 + group[i]] = mean[i];
+        if (p.rstd) p.rstd[(int64_t)w.n * p.G + w.g0 + group[i]] = rstd[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) gamma[i] *= rstd[UNI ? 0 : i];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int q = w.row + r * p.rows;
+    if (q >= p.P) break;
+    float v[VEC];
+    V::widen(raw[r], v);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) v[i] = gn_act((v[i] - mean[UNI ? 0 : i]) * gamma[i] + beta[i], p.act);
+    gn_store_any<VEC>(p.out, w.n * p.image + w.c + (int64_t)q * p.pixel, p.y_dtype, v);
+  }
+}
+
+template <class XT, int VEC, bool UNI>
+static void launch_held(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)p.N * p.tiles)), block((unsigned)plan.threads);
+  if (plan.held <= 2) hipLaunchKernelGGL((amos_gn_held<XT, VEC, 2, UNI>), grid, block, plan.lds, stream, p);
+  else if (plan.held <= 7) hipLaunchKernelGGL((amos_gn_held<XT, VEC, 7, UNI>), grid, block, plan.lds, stream, p);
+  else hipLaunchKernelGGL((amos_gn_held<XT, VEC, kGnHeldForward, UNI>), grid, block, plan.lds, stream, p);
+}
+template <class XT>
+static void pick_held(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
+  if constexpr (XT::ES == 2) {
+    if (plan.vec == 8) return plan.uni ? launch_held<XT, 8, true>(p, plan, stream) : launch_held<XT, 8, false>(p, plan, stream);
+  }
+  if (plan.vec == 4) return plan.uni ? launch_held<XT, 4, true>(p, plan, stream) : launch_held<XT, 4, false>(p, plan, stream);
+  launch_held<XT, 1, true>(p, plan, stream);
 }
 
 template <class XT, class YT, int VEC>
@@ -155,7 +274,8 @@ static void launch(const GnParams& p, hipStream_t stream) {
 }
 template <class XT, class YT>
 static void pick_vec(const GnParams& p, int vec, hipStream_t stream) {
-  if (vec == 8) launch<XT, YT, 8>(p, stream);
+  constexpr int WIDE = XT::ES == 4 || YT::ES == 4 ? 4 : 8;   // 16 bytes of the wider type
+  if (vec == WIDE) launch<XT, YT, WIDE>(p, stream);
   else launch<XT, YT, 1>(p, stream);
 }
 template <class XT>
@@ -169,17 +289,26 @@ static int run_forward(const amos_group_norm_desc_t* d, const void* x, const voi
                        void* workspace, size_t ws_bytes, hipStream_t stream) {
   GnParams p;
   GnPlan plan;
-  int rc = gn_plan(d, {x, y}, weight, bias, p, plan);
-  if (rc) return rc;
-  rc = gn_workspace(plan, p, false, workspace, ws_bytes);
+  bool wide;
+  int rc = gn_check(d, {x, y}, weight, bias, p, wide);
+  if (rc == 0) rc = gn_choose(d, false, wide, p, plan);
+  if (rc == 0) rc = gn_workspace(plan, p, workspace, ws_bytes);
   if (rc) return rc;
   p.x = x;
   p.out = y;
   p.mean = mean;
   p.rstd = rstd;
-  if (d->x_dtype == AMOS_F32) pick_out<TypeF32>(p, plan.vec, d->y_dtype, stream);
-  else if (d->x_dtype == AMOS_F16) pick_out<TypeF16>(p, plan.vec, d->y_dtype, stream);
-  else pick_out<TypeBF16>(p, plan.vec, d->y_dtype, stream);
+  if (plan.held) {
+    if (d->x_dtype == AMOS_F32) pick_held<TypeF32>(p, plan, stream);
+    else if (d->x_dtype == AMOS_F16) pick_held<TypeF16>(p, plan, stream);
+    else pick_held<TypeBF16>(p, plan, stream);
+  } else if (d->x_dtype == AMOS_F32) {
+    pick_out<TypeF32>(p, plan.vec, d->y_dtype, stream);
+  } else if (d->x_dtype == AMOS_F16) {
+    pick_out<TypeF16>(p, plan.vec, d->y_dtype, stream);
+  } else {
+    pick_out<TypeBF16>(p, plan.vec, d->y_dtype, stream);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(AMOS_ERR_HIP, "launch failed: %s", hipGetErrorString(e));
   return 0;

@@ -1,4 +1,4 @@
-// Argument checks and the plan (tiles, chunks, workspace) of the group norm launches.
+// Argument checks and the plan (kernel, tiles, chunks, workspace) of the group norm launches.
 #pragma once
 #include <string.h>
 
@@ -9,7 +9,50 @@
 
 namespace amos {
 
-inline int gn_tiles(const amos_group_norm_desc_t* d, int vec, GnParams& p, GnPlan& plan) {
+constexpr int kGnHeldForward = 16, kGnHeldGradient = 6;   // vectors a thread of the one-launch kernels holds at most
+constexpr int kGnHeldThreads = 1024;
+
+// The one-launch plan: as many groups a slab as bring a pixel's piece to 64 bytes (half a memory line), where
+// a workgroup's registers hold that much.
+inline bool gn_plan_held(const amos_group_norm_desc_t* d, bool gradient, int vec, GnParams& p, GnPlan& plan) {
+  const int es = dense_size(d->x_dtype), most = gradient ? kGnHeldGradient : kGnHeldForward;
+  int64_t unit = p.cpg;
+  while (unit % vec) unit += p.cpg;   // whole groups and whole vectors
+  if (p.C % unit) return false;
+  const auto fits = [&](int64_t c) {
+    const int64_t cols = c / vec;
+    if (cols > kGnHeldThreads) return false;
+    const int64_t rows = kGnHeldThreads / cols;
+    return (p.P + rows - 1) / rows <= most;
+  };
+  if (!fits(unit)) return false;
+  int64_t ct = unit;
+  for (int64_t k = 2; ct * es < 64 && k * unit <= p.C && k <= 64; ++k)
+    if (p.C % (k * unit) == 0 && fits(k * unit)) ct = k * unit;
+  if (p.N * (p.C / ct) >= (int64_t)1 << 31) return false;
+  p.ct = (int)ct;
+  p.tiles = (int)(p.C / ct);
+  p.sub = p.chunks = 1;
+  p.chunk = p.P;
+  p.cols = (int)(ct / vec);
+  const int rows = kGnHeldThreads / p.cols;
+  p.rows = p.P < rows ? p.P : rows;
+  plan.vec = vec;
+  plan.uni = p.cpg % vec == 0;
+  plan.held = (p.P + p.rows - 1) / p.rows;
+  plan.threads = (p.rows * p.cols + 63) / 64 * 64;
+  const int per = plan.uni && !gradient ? p.cols : (int)ct;   // values of a row of threads that meet in LDS
+  p.by_epg = make_fast_div((uint32_t)(per / (p.ct / p.cpg)));
+  p.by_cols = make_fast_div((uint32_t)p.cols);
+  p.by_cpg = make_fast_div((uint32_t)p.cpg);
+  plan.lds = (p.rows * per * (gradient ? 2 : 1) + 2 * (p.ct / p.cpg)) * (int)sizeof(float);
+  plan.part_floats = 0;
+  plan.cpart_floats = gradient && p.N > 1 ? (int64_t)p.N * p.C * 2 : 0;   // the images' shares of dweight and dbias
+  return plan.lds <= 96 * 1024;
+}
+
+// The two-launch plan; 1: this vector length does not divide the tiles
+inline int gn_plan_tiles(const amos_group_norm_desc_t* d, bool gradient, int vec, GnParams& p, GnPlan& plan) {
   const int64_t most = (int64_t)kGnThreads * vec;   // channels a workgroup can lay side by side
   const int64_t C = d->C, cpg = C / d->groups;
   int64_t ct, tiles, sub = 1;
@@ -33,17 +76,18 @@ inline int gn_tiles(const amos_group_norm_desc_t* d, int vec, GnParams& p, GnPla
   }
   if (tiles > 65535) return set_error(AMOS_ERR_UNSUPPORTED, "group norm of %lld channels in %d groups", (long long)C, d->groups);
   plan.vec = vec;
+  plan.held = 0;
   p.ct = (int)ct;
   p.tiles = (int)tiles;
   p.sub = (int)sub;
   p.cols = (int)((ct + vec - 1) / vec);
   p.rows = kGnThreads / p.cols;
-  // chunks: some 2048 workgroups, each thread at least eight pixels, at most 128 partial results to join
+  // chunks: some 2048 workgroups, each thread at least four pixels, at most 128 partial results to join
   const int64_t P = p.P;
   int64_t chunks = 2048 / (d->N * tiles);
   chunks = chunks < 1 ? 1 : chunks > 128 ? 128 : chunks;
   int64_t chunk = (P + chunks - 1) / chunks;
-  if (chunk < 8 * p.rows) chunk = 8 * p.rows;
+  if (chunk < 4 * p.rows) chunk = 4 * p.rows;
   if (chunk > P) chunk = P;
   p.chunk = (int)chunk;
   p.chunks = (int)((P + chunk - 1) / chunk);
@@ -51,13 +95,23 @@ inline int gn_tiles(const amos_group_norm_desc_t* d, int vec, GnParams& p, GnPla
   p.slots = p.chunks * p.sub;
   p.by_cols = make_fast_div((uint32_t)p.cols);
   p.by_cpg = make_fast_div((uint32_t)p.cpg);
-  plan.part_floats = (int64_t)p.N * p.G * p.slots * 3;
-  plan.cpart_floats = (int64_t)p.N * p.chunks * p.C * 2;
+  plan.part_floats = (int64_t)p.N * p.G * p.slots * (gradient ? 2 : 3);
+  plan.cpart_floats = gradient ? (int64_t)p.N * p.chunks * p.C * 2 : 0;
   return 0;
 }
 
-inline int gn_plan(const amos_group_norm_desc_t* d, std::initializer_list<const void*> tensors, const void* weight, const void* bias, GnParams& p,
-                   GnPlan& plan) {
+// `wide`: all tensors are 16-byte aligned
+inline int gn_choose(const amos_group_norm_desc_t* d, bool gradient, bool wide, GnParams& p, GnPlan& plan) {
+  const int vec = d->x_dtype == AMOS_F32 || d->y_dtype == AMOS_F32 ? 4 : 8;   // 16 bytes of the wider type
+  if (wide && d->C % vec == 0 && gn_plan_held(d, gradient, vec, p, plan)) return 0;
+  if (!(wide && d->C % 8 == 0) && gn_plan_held(d, gradient, 1, p, plan)) return 0;
+  int rc = wide ? gn_plan_tiles(d, gradient, vec, p, plan) : 1;
+  if (rc == 1) rc = gn_plan_tiles(d, gradient, 1, p, plan);
+  return rc;
+}
+
+inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<const void*> tensors, const void* weight, const void* bias, GnParams& p,
+                    bool& wide) {
   if (!d) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
   for (const void* t : tensors)
     if (!t) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
@@ -86,38 +140,36 @@ inline int gn_plan(const amos_group_norm_desc_t* d, std::initializer_list<const 
   p.eps = d->eps;
   p.act = d->activation;
   p.affine_dtype = d->affine_dtype;
+  p.y_dtype = d->y_dtype;
   p.weight = weight;
   p.bias = bias;
   const int es = dense_size(d->x_dtype) < dense_size(d->y_dtype) ? dense_size(d->x_dtype) : dense_size(d->y_dtype);
-  bool wide = true;
+  wide = true;
   for (const void* t : tensors) {
     if ((uintptr_t)t & (es - 1)) return set_error(AMOS_ERR_BAD_ARG, "group norm: misaligned tensor");
     wide = wide && ((uintptr_t)t & 15) == 0;
   }
-  int rc = wide ? gn_tiles(d, 8, p, plan) : 1;
-  if (rc == 1) rc = gn_tiles(d, 1, p, plan);
-  return rc;
+  return 0;
 }
 
-inline size_t gn_plan_bytes(const GnPlan& plan, bool gradient) {
-  return (size_t)(plan.part_floats + (gradient ? plan.cpart_floats : 0)) * sizeof(float);
-}
-// enough for the vector kernels and for the element-wise ones (the choice goes by the pointers)
+inline size_t gn_plan_bytes(const GnPlan& plan) { return (size_t)(plan.part_floats + plan.cpart_floats) * sizeof(float); }
+// enough for whatever kernel the pointers' alignment leads to
 inline size_t gn_workspace_bytes(const amos_group_norm_desc_t* d, bool gradient) {
   GnParams p;
   GnPlan plan;
-  if (gn_plan(d, {}, nullptr, nullptr, p, plan)) return 0;
-  size_t need = gn_plan_bytes(plan, gradient);
-  if (plan.vec != 1 && gn_tiles(d, 1, p, plan) == 0) {
-    const size_t other = gn_plan_bytes(plan, gradient);
-    need = other > need ? other : need;
+  bool wide;
+  if (gn_check(d, {}, nullptr, nullptr, p, wide)) return 0;
+  size_t need = 0;
+  for (const bool aligned : {true, false}) {
+    if (gn_choose(d, gradient, aligned, p, plan)) return 0;
+    need = gn_plan_bytes(plan) > need ? gn_plan_bytes(plan) : need;
   }
   return need;
 }
 
-inline int gn_workspace(const GnPlan& plan, GnParams& p, bool gradient, void* workspace, size_t ws_bytes) {
-  const size_t need = gn_plan_bytes(plan, gradient);
-  if (!workspace || ws_bytes < need || ((uintptr_t)workspace & 3))
+inline int gn_workspace(const GnPlan& plan, GnParams& p, void* workspace, size_t ws_bytes) {
+  const size_t need = gn_plan_bytes(plan);
+  if (need && (!workspace || ws_bytes < need || ((uintptr_t)workspace & 3)))
     return set_error(AMOS_ERR_WORKSPACE, "group norm: %zu bytes of workspace wanted (amos_group_norm_workspace_bytes)", need);
   p.part = (float*)workspace;
   p.cpart = p.part + plan.part_floats;

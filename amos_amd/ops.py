@@ -473,14 +473,24 @@ class Mxfp4(object):
     def __init__(self, codes, scales, cols):
         _need_device(codes, scales)
         pitch = mxfp4_pitch(cols)
-        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        rows = codes.shape[0] if codes.dim() == 2 else 0
+        if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
             raise ValueError("codes and scales are uint8, got %s and %s" % (codes.dtype, scales.dtype))
-        if codes.dim() != 2 or codes.shape[0] < 1 or codes.shape[1] != pitch or tuple(scales.shape) != (codes.shape[0], pitch // 16):
+        if rows < 1 or codes.shape != (rows, pitch) or scales.shape != (rows, pitch // 16):
             raise ValueError("%d columns want codes [rows, %d] and scales [rows, %d], got %s and %s"
                              % (cols, pitch, pitch // 16, tuple(codes.shape), tuple(scales.shape)))
         if codes.device != scales.device:
             raise ValueError("codes are on %s, scales on %s" % (codes.device, scales.device))
-        self.codes, self.scales, self.shape = codes, scales, (codes.shape[0], int(cols))
+        self.codes, self.scales, self.shape = codes, scales, (rows, int(cols))
+
+    @classmethod
+    def _empty(cls, rows, cols, like):
+        pitch = mxfp4_pitch(cols)
+        q = cls.__new__(cls)
+        q.codes = like.new_empty((rows, pitch), dtype=torch.uint8)
+        q.scales = like.new_empty((rows, pitch // 16), dtype=torch.uint8)
+        q.shape = (rows, cols)
+        return q
 
     @property
     def device(self):
@@ -507,25 +517,31 @@ def _float_code(what, dtype):
     return code
 
 
+_current_device = torch.cuda.current_device
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # absent from a build without a GPU runtime
+
+
 class _on(object):
     """The device of a call's tensors made the current one, and the stream it launches on made
-    current there, so that what the call allocates belongs to that stream's pool."""
+    current there, so that what the call allocates belongs to that stream's pool.  Entering gives the
+    stream's handle."""
 
-    __slots__ = ("guards",)
+    __slots__ = ("guards", "index")
 
     def __init__(self, device, stream):
-        self.guards = []
-        if device.index != torch.cuda.current_device():
-            self.guards.append(torch.cuda.device(device))
-        if stream is not None:
-            if stream.device != device:
-                raise ValueError("the stream belongs to %s, the tensors are on %s" % (stream.device, device))
-            self.guards.append(torch.cuda.stream(stream))
+        self.guards = ()
+        self.index = device.index
+        if stream is not None or self.index != _current_device():
+            self.guards = [torch.cuda.device(device)]
+            if stream is not None:
+                if stream.device != device:
+                    raise ValueError("the stream belongs to %s, the tensors are on %s" % (stream.device, device))
+                self.guards.append(torch.cuda.stream(stream))
 
     def __enter__(self):
         for g in self.guards:
             g.__enter__()
-        return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
         for g in reversed(self.guards):
@@ -536,7 +552,7 @@ class _on(object):
 def _scratch(need, device):
     """device scratch from the current stream's pool: (tensor, 256-byte aligned pointer)"""
     ws = torch.empty(need + 255, dtype=torch.uint8, device=device)
-    return ws, (ws.data_ptr() + 255) // 256 * 256
+    return ws, (ws.data_ptr() + 255) & ~255
 
 
 def _like_check(what, t, shape, device):
@@ -563,9 +579,7 @@ def mxfp4_quantize(x, axis=1, out=None, stream=None):
         raise ValueError("out must be an Mxfp4 of shape %s on %s, got %r" % ((rows, cols), x.device, out))
     with _on(x.device, stream) as s:
         if out is None:
-            pitch = mxfp4_pitch(cols)
-            out = Mxfp4(torch.empty((rows, pitch), dtype=torch.uint8, device=x.device),
-                        torch.empty((rows, pitch // 16), dtype=torch.uint8, device=x.device), cols)
+            out = Mxfp4._empty(rows, cols, x)
         d = _lib.Mxfp4Desc(x.shape[0], x.shape[1], code, axis)
         check(_lib.load().amos_mxfp4_quantize(ctypes.byref(d), x.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), s))
     return out
@@ -581,7 +595,7 @@ def mxfp4_dequantize(q, dtype=torch.float32, out=None, stream=None):
     code = _float_code("the result", dtype)
     with _on(q.device, stream) as s:
         if out is None:
-            out = torch.empty(q.shape, dtype=dtype, device=q.device)
+            out = q.codes.new_empty(q.shape, dtype=dtype)
         d = _lib.Mxfp4Desc(q.shape[0], q.shape[1], code, 1)
         check(_lib.load().amos_mxfp4_dequantize(ctypes.byref(d), q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), s))
     return out
@@ -680,7 +694,8 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, lay
             out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
         mean = rstd = None
         if stats:
-            mean, rstd = torch.empty((2, d.N, groups), dtype=torch.float32, device=x.device).unbind(0)
+            mean = x.new_empty((d.N, groups), dtype=torch.float32)
+            rstd = x.new_empty((d.N, groups), dtype=torch.float32)
         need = lib.amos_group_norm_workspace_bytes(ctypes.byref(d), 0)
         ws, ws_ptr = _scratch(need, x.device) if need else (None, None)
         check(lib.amos_group_norm(ctypes.byref(d), x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), _ptr(mean), _ptr(rstd),
