@@ -177,6 +177,7 @@ __global__ __launch_bounds__(1024) void amos_gn_held(const GnParams p) {
   if (w.active) {
 #pragma unroll
     for (int r = 0; r < R; ++r) {   // (pixels past the end: the last one again, left out of the sums)
+      if (r * p.rows >= p.P) break;
       const int q = w.row + r * p.rows;
       raw[r] = V::read(x + (int64_t)(q < p.P ? q : p.P - 1) * p.pixel);
     }
@@ -253,8 +254,7 @@ __global__ __launch_bounds__(1024) void amos_gn_held(const GnParams p) {
 template <class XT, int VEC, bool UNI>
 static void launch_held(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)p.N * p.tiles)), block((unsigned)plan.threads);
-  if (plan.held <= 2) hipLaunchKernelGGL((amos_gn_held<XT, VEC, 2, UNI>), grid, block, plan.lds, stream, p);
-  else if (plan.held <= 7) hipLaunchKernelGGL((amos_gn_held<XT, VEC, 7, UNI>), grid, block, plan.lds, stream, p);
+  if (plan.held <= 4) hipLaunchKernelGGL((amos_gn_held<XT, VEC, 4, UNI>), grid, block, plan.lds, stream, p);
   else hipLaunchKernelGGL((amos_gn_held<XT, VEC, kGnHeldForward, UNI>), grid, block, plan.lds, stream, p);
 }
 template <class XT>

@@ -521,44 +521,44 @@ _current_device = torch.cuda.current_device
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # absent from a build without a GPU runtime
 
 
-class _on(object):
-    """The device of a call's tensors made the current one, and the stream it launches on made
-    current there, so that what the call allocates belongs to that stream's pool.  Entering gives the
-    stream's handle."""
-
-    __slots__ = ("guards", "index")
-
-    def __init__(self, device, stream):
-        self.guards = ()
-        self.index = device.index
-        if stream is not None or self.index != _current_device():
-            self.guards = [torch.cuda.device(device)]
-            if stream is not None:
-                if stream.device != device:
-                    raise ValueError("the stream belongs to %s, the tensors are on %s" % (stream.device, device))
-                self.guards.append(torch.cuda.stream(stream))
-
-    def __enter__(self):
-        for g in self.guards:
-            g.__enter__()
-        return _raw_stream(self.index)
-
-    def __exit__(self, *exc):
-        for g in reversed(self.guards):
-            g.__exit__(*exc)
-        return False
+def _on(body, device, stream, *args):
+    """body(handle of the stream to launch on, *args) with `device` the current one and `stream` (None: the
+    device's current one) current there, so that what the call allocates belongs to that stream's pool"""
+    index = device.index
+    if stream is None:
+        if index == _current_device():
+            return body(_raw_stream(index), *args)
+        with torch.cuda.device(device):
+            return body(_raw_stream(index), *args)
+    if stream.device != device:
+        raise ValueError("the stream belongs to %s, the tensors are on %s" % (stream.device, device))
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        return body(stream.cuda_stream, *args)
 
 
-def _scratch(need, device):
+def _scratch(need, like):
     """device scratch from the current stream's pool: (tensor, 256-byte aligned pointer)"""
-    ws = torch.empty(need + 255, dtype=torch.uint8, device=device)
+    ws = like.new_empty(need + 255, dtype=torch.uint8)
     return ws, (ws.data_ptr() + 255) & ~255
 
 
 def _like_check(what, t, shape, device):
     _need_device(t)
-    if tuple(t.shape) != tuple(shape) or t.device != device:
+    if t.shape != shape or t.device != device:
         raise ValueError("%s must be of shape %s on %s, got %s on %s" % (what, tuple(shape), device, tuple(t.shape), t.device))
+
+
+class _Plans(dict):
+    """what follows from a call's shapes and types alone (checked descriptor, workspace bytes), by these"""
+
+    def keep(self, key, plan):
+        if len(self) >= 4096:
+            self.clear()
+        self[key] = plan
+        return plan
+
+
+_MX_GEMM_PLANS, _NORM_PLANS = _Plans(), _Plans()
 
 
 def mxfp4_quantize(x, axis=1, out=None, stream=None):
@@ -573,15 +573,19 @@ def mxfp4_quantize(x, axis=1, out=None, stream=None):
     if axis not in (0, 1, -1, -2):
         raise ValueError("axis %s of a matrix" % (axis,))
     axis = axis % 2
-    code = _float_code("x", x.dtype)
-    rows, cols = x.shape if axis else (x.shape[1], x.shape[0])
+    rows, cols = x.shape
+    d = _lib.Mxfp4Desc(rows, cols, _float_code("x", x.dtype), axis)
+    if axis == 0:
+        rows, cols = cols, rows
     if out is not None and (not isinstance(out, Mxfp4) or out.shape != (rows, cols) or out.device != x.device):
         raise ValueError("out must be an Mxfp4 of shape %s on %s, got %r" % ((rows, cols), x.device, out))
-    with _on(x.device, stream) as s:
-        if out is None:
-            out = Mxfp4._empty(rows, cols, x)
-        d = _lib.Mxfp4Desc(x.shape[0], x.shape[1], code, axis)
-        check(_lib.load().amos_mxfp4_quantize(ctypes.byref(d), x.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), s))
+    return _on(_quantize, x.device, stream, x, d, rows, cols, out)
+
+
+def _quantize(s, x, d, rows, cols, out):
+    if out is None:
+        out = Mxfp4._empty(rows, cols, x)
+    check(_lib.load().amos_mxfp4_quantize(ctypes.byref(d), x.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), s))
     return out
 
 
@@ -592,12 +596,14 @@ def mxfp4_dequantize(q, dtype=torch.float32, out=None, stream=None):
     if out is not None:
         _need_device(out)
         _check_out(out, q.shape, dtype, q.codes)
-    code = _float_code("the result", dtype)
-    with _on(q.device, stream) as s:
-        if out is None:
-            out = q.codes.new_empty(q.shape, dtype=dtype)
-        d = _lib.Mxfp4Desc(q.shape[0], q.shape[1], code, 1)
-        check(_lib.load().amos_mxfp4_dequantize(ctypes.byref(d), q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), s))
+    d = _lib.Mxfp4Desc(q.shape[0], q.shape[1], _float_code("the result", dtype), 1)
+    return _on(_dequantize, q.codes.device, stream, q, d, dtype, out)
+
+
+def _dequantize(s, q, d, dtype, out):
+    if out is None:
+        out = q.codes.new_empty(q.shape, dtype=dtype)
+    check(_lib.load().amos_mxfp4_dequantize(ctypes.byref(d), q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), s))
     return out
 
 
@@ -607,65 +613,89 @@ def mxfp4_gemm(a, b, out=None, out_dtype=torch.float32, add=None, bias=None, str
     mxfp4_quantize does.  fp32 accumulation, one rounding to the output's type; `add` may be `out`."""
     if not isinstance(b, Mxfp4):
         raise ValueError("b must be an Mxfp4, got %s" % type(b))
+    device = b.codes.device
     dense = not isinstance(a, Mxfp4)
     if dense:
         _need_device(a)
-        a_code = _float_code("a", a.dtype)
-    else:
-        a_code = _lib.AMOS_MXFP4
-    if len(a.shape) != 2 or a.shape[0] < 1 or a.shape[1] != b.shape[1] or a.device != b.device:
-        raise ValueError("operands do not agree: a %s on %s, b %s on %s" % (tuple(a.shape), a.device, b.shape, b.device))
-    M, N, K = a.shape[0], b.shape[0], b.shape[1]
+    if a.device != device:
+        raise ValueError("a is on %s, b on %s" % (a.device, device))
     if out is not None:
         out_dtype = out.dtype
-        _like_check("out", out, (M, N), b.device)
-    d = _lib.Mxfp4GemmDesc(M, N, K, a_code, _float_code("the output", out_dtype))
+    key = (a.shape, b.shape, a.dtype if dense else None, out_dtype)
+    plan = _MX_GEMM_PLANS.get(key) or _MX_GEMM_PLANS.keep(key, _mxfp4_gemm_plan(*key))
+    if out is not None:
+        _like_check("out", out, plan[1], device)
     epi = None
     if add is not None or bias is not None:
         epi = _lib.Mxfp4Epilogue()
         if bias is not None:
-            _like_check("bias", bias, (N,), b.device)
+            _like_check("bias", bias, plan[1][1:], device)
             epi.bias, epi.bias_dtype = bias.data_ptr(), _float_code("bias", bias.dtype)
         if add is not None:
-            _like_check("the added operand", add, (M, N), b.device)
+            _like_check("the added operand", add, plan[1], device)
             epi.add, epi.add_dtype = add.data_ptr(), _float_code("the added operand", add.dtype)
-    lib = _lib.load()
-    with _on(b.device, stream) as s:
-        if out is None:
-            out = torch.empty((M, N), dtype=out_dtype, device=b.device)
-        need = lib.amos_mxfp4_gemm_workspace_bytes(ctypes.byref(d))
-        ws, ws_ptr = _scratch(need, b.device) if need else (None, None)
-        ac, asc = (a.data_ptr(), None) if dense else (a.codes.data_ptr(), a.scales.data_ptr())
-        check(lib.amos_mxfp4_gemm(ctypes.byref(d), None if epi is None else ctypes.byref(epi), ac, asc, b.codes.data_ptr(),
-                                  b.scales.data_ptr(), out.data_ptr(), ws_ptr, need, s))
+        epi = ctypes.byref(epi)
+    return _on(_mxfp4_gemm, device, stream, plan, a, b, dense, out, out_dtype, epi)
+
+
+def _mxfp4_gemm_plan(a_shape, b_shape, a_dtype, out_dtype):
+    """(descriptor, shape of the result, workspace bytes)"""
+    if len(a_shape) != 2 or a_shape[0] < 1 or a_shape[1] != b_shape[1]:
+        raise ValueError("operands do not agree: a %s, b %s" % (tuple(a_shape), b_shape))
+    d = _lib.Mxfp4GemmDesc(a_shape[0], b_shape[0], b_shape[1], _lib.AMOS_MXFP4 if a_dtype is None else _float_code("a", a_dtype),
+                           _float_code("the output", out_dtype))
+    need = _lib.load().amos_mxfp4_gemm_workspace_bytes(ctypes.byref(d))
+    return d, (a_shape[0], b_shape[0]), need
+
+
+def _mxfp4_gemm(s, plan, a, b, dense, out, out_dtype, epi):
+    d, shape, need = plan
+    if out is None:
+        out = b.codes.new_empty(shape, dtype=out_dtype)
+    ws, ws_ptr = _scratch(need, b.codes) if need else (None, None)
+    ac, asc = (a.data_ptr(), None) if dense else (a.codes.data_ptr(), a.scales.data_ptr())
+    check(_lib.load().amos_mxfp4_gemm(ctypes.byref(d), epi, ac, asc, b.codes.data_ptr(), b.scales.data_ptr(), out.data_ptr(), ws_ptr, need, s))
     return out
 
 
 _ACT_CODE = {None: _lib.AMOS_ACT_NONE, "none": _lib.AMOS_ACT_NONE, "relu": _lib.AMOS_ACT_RELU, "silu": _lib.AMOS_ACT_SILU}
 
 
-def _group_norm_desc(x, groups, weight, bias, eps, activation, layout, out_dtype):
+def _group_norm_plan(gradient, x_shape, x_dtype, y_dtype, groups, weight_dtype, bias_dtype, eps, activation, layout):
+    """(descriptor, workspace bytes, shape of the coefficients, shape of the statistics)"""
     code = _lib.LAYOUT_CODE.get(layout)
     if code not in (_lib.AMOS_LAYOUT_NHWC, _lib.AMOS_LAYOUT_HWNC):
         raise ValueError("group norm runs on the channels-last layouts (nhwc, ndhwc, hwnc, dhwnc), got %r" % (layout,))
-    if x.dim() != len(layout) or x.numel() == 0:
-        raise ValueError("layout %s wants a tensor of %d dimensions with elements, got shape %s" % (layout, len(layout), tuple(x.shape)))
+    if len(x_shape) != len(layout) or 0 in x_shape:
+        raise ValueError("layout %s wants a tensor of %d dimensions with elements, got shape %s" % (layout, len(layout), tuple(x_shape)))
     if activation not in _ACT_CODE:
         raise ValueError("activation is None, 'relu' or 'silu', got %r" % (activation,))
-    ext = dict(zip(layout, x.shape))
+    ext = dict(zip(layout, x_shape))
     if groups < 1 or ext["c"] % groups:
         raise ValueError("%d channels in %d groups" % (ext["c"], groups))
+    if weight_dtype is not None and bias_dtype is not None and weight_dtype != bias_dtype:
+        raise ValueError("weight is %s, bias %s" % (weight_dtype, bias_dtype))
     d = _lib.GroupNormDesc()
     d.N, d.C, d.D, d.H, d.W = ext["n"], ext["c"], ext.get("d", 1), ext["h"], ext["w"]
     d.groups, d.activation, d.layout, d.eps = groups, _ACT_CODE[activation], code, eps
-    d.x_dtype, d.y_dtype = _float_code("x", x.dtype), _float_code("the output", out_dtype)
-    for what, t in (("weight", weight), ("bias", bias)):
+    d.x_dtype, d.y_dtype = _float_code("x", x_dtype), _float_code("the output", y_dtype)
+    for t in (weight_dtype, bias_dtype):
         if t is not None:
-            _like_check(what, t, (ext["c"],), x.device)
-            d.affine_dtype = _float_code(what, t.dtype)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError("weight is %s, bias %s" % (weight.dtype, bias.dtype))
-    return d
+            d.affine_dtype = _float_code("weight and bias", t)
+    need = _lib.load().amos_group_norm_workspace_bytes(ctypes.byref(d), int(gradient))
+    return d, need, (ext["c"],), (ext["n"], groups)
+
+
+def _group_norm_key(gradient, x, y_dtype, groups, weight, bias, eps, activation, layout):
+    """the plan of a call, its coefficients checked"""
+    key = (gradient, x.shape, x.dtype, y_dtype, groups, None if weight is None else weight.dtype, None if bias is None else bias.dtype, eps,
+           activation, layout)
+    plan = _NORM_PLANS.get(key) or _NORM_PLANS.keep(key, _group_norm_plan(*key))
+    if weight is not None:
+        _like_check("weight", weight, plan[2], x.device)
+    if bias is not None:
+        _like_check("bias", bias, plan[2], x.device)
+    return plan
 
 
 def _ptr(t):
@@ -687,19 +717,19 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, lay
         out_dtype = out.dtype
     elif out_dtype is None:
         out_dtype = x.dtype
-    d = _group_norm_desc(x, groups, weight, bias, eps, activation, layout, out_dtype)
-    lib = _lib.load()
-    with _on(x.device, stream) as s:
-        if out is None:
-            out = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-        mean = rstd = None
-        if stats:
-            mean = x.new_empty((d.N, groups), dtype=torch.float32)
-            rstd = x.new_empty((d.N, groups), dtype=torch.float32)
-        need = lib.amos_group_norm_workspace_bytes(ctypes.byref(d), 0)
-        ws, ws_ptr = _scratch(need, x.device) if need else (None, None)
-        check(lib.amos_group_norm(ctypes.byref(d), x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), _ptr(mean), _ptr(rstd),
-                                  ws_ptr, need, s))
+    plan = _group_norm_key(False, x, out_dtype, groups, weight, bias, eps, activation, layout)
+    return _on(_group_norm, x.device, stream, plan, x, weight, bias, out, out_dtype, stats)
+
+
+def _group_norm(s, plan, x, weight, bias, out, out_dtype, stats):
+    d, need, _, stats_shape = plan
+    if out is None:
+        out = x.new_empty(x.shape, dtype=out_dtype)
+    mean = rstd = None
+    if stats:
+        mean, rstd = x.new_empty(stats_shape, dtype=torch.float32), x.new_empty(stats_shape, dtype=torch.float32)
+    ws, ws_ptr = _scratch(need, x) if need else (None, None)
+    check(_lib.load().amos_group_norm(ctypes.byref(d), x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), _ptr(mean), _ptr(rstd), ws_ptr, need, s))
     return (out, mean, rstd) if stats else out
 
 
@@ -709,20 +739,21 @@ def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, activ
     _need_device(dy, x, mean, rstd)
     if dy.shape != x.shape or dy.device != x.device:
         raise ValueError("dy is %s on %s, x %s on %s" % (tuple(dy.shape), dy.device, tuple(x.shape), x.device))
-    d = _group_norm_desc(x, groups, weight, bias, 0.0, activation, layout, dy.dtype)
+    plan = _group_norm_key(True, x, dy.dtype, groups, weight, bias, 0.0, activation, layout)
     for what, t in (("mean", mean), ("rstd", rstd)):
-        _like_check(what, t, (d.N, groups), x.device)
-        if t.dtype != torch.float32:
-            raise ValueError("%s is fp32, got %s" % (what, t.dtype))
-    lib = _lib.load()
-    with _on(x.device, stream) as s:
-        dx = torch.empty_like(x)
-        dweight = None if weight is None else torch.empty(d.C, dtype=torch.float32, device=x.device)
-        dbias = None if bias is None else torch.empty(d.C, dtype=torch.float32, device=x.device)
-        need = lib.amos_group_norm_workspace_bytes(ctypes.byref(d), 1)
-        ws, ws_ptr = _scratch(need, x.device) if need else (None, None)
-        check(lib.amos_group_norm_backward(ctypes.byref(d), dy.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias), mean.data_ptr(),
-                                           rstd.data_ptr(), dx.data_ptr(), _ptr(dweight), _ptr(dbias), ws_ptr, need, s))
+        if t.shape != plan[3] or t.device != x.device or t.dtype != torch.float32:
+            raise ValueError("%s must be fp32 of shape %s on %s, got %s %s on %s" % (what, plan[3], x.device, t.dtype, tuple(t.shape), t.device))
+    return _on(_group_norm_backward, x.device, stream, plan, dy, x, mean, rstd, weight, bias)
+
+
+def _group_norm_backward(s, plan, dy, x, mean, rstd, weight, bias):
+    d, need, coefficients, _ = plan
+    dx = x.new_empty(x.shape)
+    dweight = None if weight is None else x.new_empty(coefficients, dtype=torch.float32)
+    dbias = None if bias is None else x.new_empty(coefficients, dtype=torch.float32)
+    ws, ws_ptr = _scratch(need, x) if need else (None, None)
+    check(_lib.load().amos_group_norm_backward(ctypes.byref(d), dy.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias), mean.data_ptr(),
+                                               rstd.data_ptr(), dx.data_ptr(), _ptr(dweight), _ptr(dbias), ws_ptr, need, s))
     return dx, dweight, dbias
 
 
