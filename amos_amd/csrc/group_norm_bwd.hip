@@ -104,12 +104,25 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_partial(const GnP
 __device__ __forceinline__ void gn_coefficient_gradients(const GnParams& p, int block, float* s1, float* s2) {
   const int t = threadIdx.x, c = block * 16 + (t & 15), r0 = t >> 4;
   const int rows = p.N * p.chunks;   // (one-launch kernel: a row an image)
+  typedef float v2f __attribute__((ext_vector_type(2)));
   float a = 0.f, b = 0.f;
   if (c < p.C) {
-    const float* at = p.cpart + (int64_t)c * 2;
-    for (int r = r0; r < rows; r += 16) {
-      a += at[(int64_t)r * p.C * 2];
-      b += at[(int64_t)r * p.C * 2 + 1];
+    const v2f* const at = (const v2f*)p.cpart + c;
+    int r = r0;
+    for (; r + 7 * 16 < rows; r += 8 * 16) {   // eight rows in flight
+      v2f v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = at[(int64_t)(r + u * 16) * p.C];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        a += v[u][0];
+        b += v[u][1];
+      }
+    }
+    for (; r < rows; r += 16) {
+      const v2f v = at[(int64_t)r * p.C];
+      a += v[0];
+      b += v[1];
     }
   }
   s1[t] = a;
@@ -126,15 +139,16 @@ __device__ __forceinline__ void gn_coefficient_gradients(const GnParams& p, int 
   }
 }
 
-// ---- second launch: dx; behind the workgroups of the tiles those of dweight and dbias ---------------
+// ---- second launch: dx; in front of the workgroups of the tiles those of dweight and dbias (`more` of them: their
+// sums are the longest chain of the launch) ----------------------------------------------------------------------
 template <class XT, class YT, int VEC>
-__global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_apply(const GnParams p) {
+__global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_apply(const GnParams p, int more) {
   __shared__ float s1[kGnThreads * VEC], s2[kGnThreads * VEC];   // by group of the tile: E[d weight], E[d weight h]
-  if ((int)blockIdx.x >= p.N * p.chunks) {
-    if (blockIdx.y == 0) gn_coefficient_gradients(p, (int)blockIdx.x - p.N * p.chunks, s1, s2);
+  if ((int)blockIdx.x < more) {
+    if (blockIdx.y == 0) gn_coefficient_gradients(p, (int)blockIdx.x, s1, s2);
     return;
   }
-  const GnTile w = gn_tile<VEC>(p, blockIdx.x);
+  const GnTile w = gn_tile<VEC>(p, (int)blockIdx.x - more);
   const GnChannels<VEC> ch(p, w.n, w.c0 + (w.active ? w.col * VEC : 0));
   {
     const int team = gn_team(w.groups), t = threadIdx.x, lane = t & (team - 1);
@@ -362,7 +376,7 @@ static void launch(const GnParams& p, hipStream_t stream) {
   const unsigned work = (unsigned)((int64_t)p.N * p.chunks);
   const unsigned more = p.dweight || p.dbias ? (unsigned)((p.C + 15) / 16) : 0;
   hipLaunchKernelGGL((amos_gn_gradient_partial<XT, YT, VEC>), dim3(work, (unsigned)p.tiles), dim3(kGnThreads), 0, stream, p);
-  hipLaunchKernelGGL((amos_gn_gradient_apply<XT, YT, VEC>), dim3(work + more, (unsigned)p.tiles), dim3(kGnThreads), 0, stream, p);
+  hipLaunchKernelGGL((amos_gn_gradient_apply<XT, YT, VEC>), dim3(work + more, (unsigned)p.tiles), dim3(kGnThreads), 0, stream, p, (int)more);
 }
 template <class XT, class YT>
 static int pick_kernel(const GnParams& p, const GnPlan& plan, hipStream_t stream) {

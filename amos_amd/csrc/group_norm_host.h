@@ -87,9 +87,9 @@ inline int gn_plan_tiles(const amos_group_norm_desc_t* d, bool gradient, int vec
   p.sub = (int)sub;
   p.cols = (int)((ct + vec - 1) / vec);
   p.rows = kGnThreads / p.cols;
-  // chunks: some 2048 workgroups, each thread at least four pixels, at most 128 partial results to join
+  // chunks: some 1024 workgroups, each thread at least four pixels, at most 128 partial results to join
   const int64_t P = p.P;
-  int64_t chunks = 2048 / (d->N * tiles);
+  int64_t chunks = 1024 / (d->N * tiles);
   chunks = chunks < 1 ? 1 : chunks > 128 ? 128 : chunks;
   int64_t chunk = (P + chunks - 1) / chunks;
   if (chunk < 4 * p.rows) chunk = 4 * p.rows;
@@ -157,7 +157,7 @@ inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<const
   return 0;
 }
 
-inline size_t gn_plan_bytes(const GnPlan& plan) { return (size_t)(plan.part_floats + plan.cpart_floats) * sizeof(float); }
+inline size_t gn_plan_bytes(const GnPlan& plan) { return (size_t)((plan.part_floats + 1) / 2 * 2 + plan.cpart_floats) * sizeof(float); }
 // enough for whatever kernel the pointers' alignment leads to
 inline size_t gn_workspace_bytes(const amos_group_norm_desc_t* d, bool gradient) {
   GnParams p;
@@ -174,10 +174,10 @@ inline size_t gn_workspace_bytes(const amos_group_norm_desc_t* d, bool gradient)
 
 inline int gn_workspace(const GnPlan& plan, GnParams& p, void* workspace, size_t ws_bytes) {
   const size_t need = gn_plan_bytes(plan);
-  if (need && (!workspace || ws_bytes < need || ((uintptr_t)workspace & 3)))
+  if (need && (!workspace || ws_bytes < need || ((uintptr_t)workspace & 7)))
     return set_error(AMOS_ERR_WORKSPACE, "group norm: %zu bytes of workspace wanted (amos_group_norm_workspace_bytes)", need);
   p.part = (float*)workspace;
-  p.cpart = p.part + plan.part_floats;
+  p.cpart = p.part + (plan.part_floats + 1) / 2 * 2;
   return 0;
 }
 

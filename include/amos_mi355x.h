@@ -444,7 +444,7 @@ typedef struct {
   int32_t reserved;
 } amos_group_norm_desc_t;
 
-/* bytes of device scratch the call wants; less: AMOS_ERR_WORKSPACE */
+/* bytes of 8-byte aligned device scratch the call wants; less: AMOS_ERR_WORKSPACE */
 size_t amos_group_norm_workspace_bytes(const amos_group_norm_desc_t* desc, int gradient);
 int amos_group_norm(const amos_group_norm_desc_t* desc, const void* x, const void* weight, const void* bias,
                     void* y, float* mean, float* rstd, void* workspace, size_t ws_bytes, void* stream);
