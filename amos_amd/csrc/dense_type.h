@@ -44,6 +44,12 @@ struct DenseVec {
     for (int i = 0; i < N; ++i) v[i] = T::widen(x[i]);
   }
   static __device__ __forceinline__ void load(const raw_t* p, float* v) { widen(read(p), v); }
+  static __device__ __forceinline__ void store_streaming(raw_t* p, const float* v) {
+    vec_t x;
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = T::narrow(v[i]);
+    __builtin_nontemporal_store(x, (vec_t*)p);
+  }
   static __device__ __forceinline__ void store(raw_t* p, const float* v) {
     vec_t x;
 #pragma unroll

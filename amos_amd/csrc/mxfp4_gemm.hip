@@ -11,11 +11,12 @@ namespace amos {
 
 // ---- few rows of A ------------------------------------------------------------------------------
 // With few tokens the weights B are read once and hardly reused: the call lasts as long as their
-// bytes take.  The weights are the matrix instruction's row operand and come from HBM straight into
-// registers (no LDS: nothing is shared), tokens are its columns.  A workgroup of eight waves owns
-// 16 RT rows of B and up to 16 TT tokens; the waves take K in turns of 512 elements (four
-// instructions' worth: 256 contiguous bytes of every row and four words of scales, all loads of a
-// turn in flight together) and their sums meet in LDS, added in the order of the waves.
+// bytes take.  The weights are the matrix instruction's row operand and come from memory straight into
+// registers (no LDS: nothing is shared), tokens are its columns.  A workgroup owns 16 RT rows of B and up
+// to 16 TT tokens; its waves take K in turns of 512 elements (four instructions' worth: 256 contiguous
+// bytes of every row), and there are as many waves, up to 16, as give each one turn: all of a wave's loads
+// are in flight together.  A row's scales of a turn are one 16-byte load.  The waves' sums meet in LDS,
+// added in the order of the waves.
 // SRC: what A is -- codes, or (fp32 / fp16 / bf16) elements that are quantised here: a lane's fragment
 // is exactly one block, so it finds the block's scale without any exchange.
 enum { SRC_MX = 0, SRC_F32 = 1, SRC_F16 = 2, SRC_BF16 = 3 };
@@ -23,15 +24,18 @@ template <int SRC> struct SrcType { typedef TypeF32 type; };
 template <> struct SrcType<SRC_F16> { typedef TypeF16 type; };
 template <> struct SrcType<SRC_BF16> { typedef TypeBF16 type; };
 
-// the block (step, lane group) of token row `m`, quantised
+// the block of token row `m` that starts at element k, quantised
 template <class T>
 __device__ __forceinline__ void mx_quantize_fragment(const MxGemmParams& p, int64_t m, int64_t k, mx_v4i& codes, int& scale) {
   const typename T::raw_t* const x = (const typename T::raw_t*)p.dense + m * p.K + k;
   float v[32];
   if (p.dense_vec && k + 32 <= p.K) {
     constexpr int N = 16 / T::ES;
+    typename DenseVec<T, N>::vec_t raw[32 / N];
 #pragma unroll
-    for (int i = 0; i < 32; i += N) DenseVec<T, N>::load(x + i, v + i);
+    for (int i = 0; i < 32 / N; ++i) raw[i] = DenseVec<T, N>::read(x + i * N);
+#pragma unroll
+    for (int i = 0; i < 32 / N; ++i) DenseVec<T, N>::widen(raw[i], v + i * N);
   } else {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = k + i < p.K ? T::widen(x[i]) : 0.f;
@@ -48,106 +52,174 @@ __device__ __forceinline__ void mx_quantize_fragment(const MxGemmParams& p, int6
   for (int i = 0; i < 4; ++i) codes[i] = (int)mx_encode8(v + 8 * i, s);
 }
 
-constexpr int kFewWaves = 8, kFewTurn = 4;
+constexpr int kTurn = 4;
+typedef int mx_v4i_words __attribute__((ext_vector_type(4), aligned(4)));
 
-template <int SRC, int RT, int TT>
-__global__ __launch_bounds__(64 * kFewWaves) void amos_mx_gemm_few(const MxGemmParams p) {
-  __shared__ __attribute__((aligned(16))) float sums[kFewWaves][RT * TT][64][4];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+// a turn of one row's fragments and scales.  `here` (uniform) of its kTurn steps exist; past them: the last step again
+__device__ __forceinline__ void mx_load_turn(const unsigned char* codes, const unsigned char* scales, int s0, int here, int q, mx_v4i* f, mx_v4i& x) {
+#pragma unroll
+  for (int u = 0; u < kTurn; ++u) f[u] = *(const mx_v4i*)(codes + (int64_t)(s0 + (u < here ? u : here - 1)) * 64 + q * 16);
+  if (here == kTurn) {
+    x = *(const mx_v4i_words*)(scales + (int64_t)s0 * 4);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kTurn; ++u) x[u] = *(const int*)(scales + (int64_t)(s0 + (u < here ? u : here - 1)) * 4);
+  }
+}
+
+template <int SRC, int RT, int TT, int MAXW>
+__global__ __launch_bounds__(64 * MAXW) void amos_mx_gemm_few(const MxGemmParams p) {
+  extern __shared__ __attribute__((aligned(16))) float sums[];   // [waves][RT * TT][64][4]
+  const int t = threadIdx.x, lane = t & 63, waves = (int)blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int r = lane & 15, q = lane >> 4;
   const int n0 = blockIdx.x * (16 * RT), m0 = blockIdx.y * (16 * TT);
   const int64_t pitch = (int64_t)p.steps * 64, spitch = (int64_t)p.steps * 4;
-  const unsigned char *brow[RT], *bsc[RT], *arow[TT], *asc[TT];
-#pragma unroll
-  for (int i = 0; i < RT; ++i) {   // (rows past the end repeat the last one: their sums are not stored)
-    const int64_t n = n0 + 16 * i + r < p.N ? n0 + 16 * i + r : p.N - 1;
-    brow[i] = p.b + n * pitch + q * 16;
-    bsc[i] = p.bs + n * spitch + q;
-  }
-#pragma unroll
-  for (int j = 0; j < TT; ++j) {
-    const int64_t m = m0 + 16 * j + r < p.M ? m0 + 16 * j + r : p.M - 1;
-    arow[j] = p.a + m * pitch + q * 16;
-    asc[j] = p.as + m * spitch + q;
-  }
   v4f acc[RT][TT];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
     for (int j = 0; j < TT; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int s0 = wave * kFewTurn; s0 < p.steps; s0 += kFewWaves * kFewTurn) {
-    mx_v4i bf[kFewTurn][RT];
-    int bx[kFewTurn][RT];
+  for (int s0 = wave * kTurn; s0 < p.steps; s0 += waves * kTurn) {
+    const int here = p.steps - s0 < kTurn ? p.steps - s0 : kTurn;
+    mx_v4i bf[RT][kTurn], bx[RT];
+    mx_v4i af[TT][kTurn], ax[TT];
 #pragma unroll
-    for (int u = 0; u < kFewTurn; ++u) {
-      const int s = s0 + u < p.steps ? s0 + u : p.steps - 1;   // (past the end: loaded again, not multiplied)
+    for (int i = 0; i < RT; ++i) {   // (rows past the end repeat the last one: their sums are not stored)
+      const int64_t n = n0 + 16 * i + r < p.N ? n0 + 16 * i + r : p.N - 1;
+      mx_load_turn(p.b + n * pitch, p.bs + n * spitch, s0, here, q, bf[i], bx[i]);
+    }
+    if constexpr (SRC == SRC_MX) {
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        bf[u][i] = *(const mx_v4i*)(brow[i] + s * 64);
-        bx[u][i] = bsc[i][s * 4];
+      for (int j = 0; j < TT; ++j) {
+        const int64_t m = m0 + 16 * j + r < p.M ? m0 + 16 * j + r : p.M - 1;
+        mx_load_turn(p.a + m * pitch, p.as + m * spitch, s0, here, q, af[j], ax[j]);
       }
     }
 #pragma unroll
-    for (int u = 0; u < kFewTurn; ++u) {
-      const int s = s0 + u;
-      if (s >= p.steps) break;
-      mx_v4i af[TT];
-      int ax[TT];
+    for (int u = 0; u < kTurn; ++u) {
+      if (u >= here) break;
+      int xa[TT];
+      if constexpr (SRC == SRC_MX) {
 #pragma unroll
-      for (int j = 0; j < TT; ++j) {
-        if constexpr (SRC == SRC_MX) {
-          af[j] = *(const mx_v4i*)(arow[j] + s * 64);
-          ax[j] = asc[j][s * 4];
-        } else {
+        for (int j = 0; j < TT; ++j) xa[j] = (int)((unsigned)ax[j][u] >> (8 * q));   // (the instruction takes the lowest byte)
+      } else {
+#pragma unroll
+        for (int j = 0; j < TT; ++j) {
           const int64_t m = m0 + 16 * j + r;
-          af[j] = mx_v4i{0, 0, 0, 0};
-          ax[j] = 0;
-          if (m < p.M) mx_quantize_fragment<typename SrcType<SRC>::type>(p, m, (int64_t)s * 128 + q * 32, af[j], ax[j]);
+          af[j][u] = mx_v4i{0, 0, 0, 0};
+          xa[j] = 0;
+          if (m < p.M) mx_quantize_fragment<typename SrcType<SRC>::type>(p, m, (int64_t)(s0 + u) * 128 + q * 32, af[j][u], xa[j]);
         }
       }
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
+      for (int i = 0; i < RT; ++i) {
+        const int xb = (int)((unsigned)bx[i][u] >> (8 * q));
 #pragma unroll
-        for (int j = 0; j < TT; ++j) acc[i][j] = mx_mfma(bf[u][i], af[j], acc[i][j], bx[u][i], ax[j]);
+        for (int j = 0; j < TT; ++j) acc[i][j] = mx_mfma(bf[i][u], af[j][u], acc[i][j], xb, xa[j]);
+      }
     }
   }
+  if (waves > 1) {
 #pragma unroll
-  for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int j = 0; j < TT; ++j) *(v4f*)sums[wave][i * TT + j][lane] = acc[i][j];
-  __syncthreads();
-  for (int slot = t; slot < RT * TT * 64; slot += 64 * kFewWaves) {
+      for (int j = 0; j < TT; ++j) *(v4f*)(sums + (((wave * RT + i) * TT + j) * 64 + lane) * 4) = acc[i][j];
+    __syncthreads();
+  }
+  // a lane's four sums: rows 4q .. 4q + 3 of B for one token, neighbours in C
+  auto finish = [&](int i, int j, int l, v4f v) {
+    const int64_t m = m0 + 16 * j + (l & 15);
+    const int n = n0 + 16 * i + 4 * (l >> 4);
+    if (m >= p.M || n >= p.N) return;
+    const int64_t at = m * p.N + n;
+    if (n + 4 <= p.N) {
+      float e[4];
+      if (p.tail.bias) {
+        load_run_any<4>(p.tail.bias, n, p.tail.bias_dtype, 0.f, e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += e[k];
+      }
+      if (p.tail.add) {
+        load_run_any<4>(p.tail.add, at, p.tail.add_dtype, 0.f, e);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] += e[k];
+      }
+      if (p.vec_out) {
+        const float w[4] = {v[0], v[1], v[2], v[3]};
+        if (p.out_dtype == AMOS_F32) DenseVec<TypeF32, 4>::store((float*)p.c + at, w);
+        else if (p.out_dtype == AMOS_F16) DenseVec<TypeF16, 4>::store((_Float16*)p.c + at, w);
+        else DenseVec<TypeBF16, 4>::store((__bf16*)p.c + at, w);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) store_any(p.c, at + k, p.out_dtype, v[k]);
+      }
+    } else {
+      for (int k = 0; k < 4 && n + k < p.N; ++k) store_any(p.c, at + k, p.out_dtype, mx_tail(p.tail, v[k], m, n + k, p.N));
+    }
+  };
+  if (waves == 1) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int j = 0; j < TT; ++j) finish(i, j, lane, acc[i][j]);
+    return;
+  }
+  for (int slot = t; slot < RT * TT * 64; slot += (int)blockDim.x) {
     const int tile = slot >> 6, l = slot & 63;
-    v4f v = *(const v4f*)sums[0][tile][l];
-#pragma unroll
-    for (int w = 1; w < kFewWaves; ++w) {
-      const v4f x = *(const v4f*)sums[w][tile][l];
+    v4f v = *(const v4f*)(sums + (tile * 64 + l) * 4);
+    for (int w = 1; w < waves; ++w) {
+      const v4f x = *(const v4f*)(sums + ((w * RT * TT + tile) * 64 + l) * 4);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] += x[e];
     }
-    const int64_t m = m0 + 16 * (tile % TT) + (l & 15);
-    const int n = n0 + 16 * (tile / TT) + 4 * (l >> 4);
-    if (m < p.M) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.N) store_any(p.c, m * p.N + n + e, p.out_dtype, mx_tail(p.tail, v[e], m, n + e, p.N));
-    }
+    finish(tile / TT, tile % TT, l, v);
   }
 }
 
-template <int RT, int TT>
-static void launch_few(const MxGemmParams& p, int src, hipStream_t stream) {
-  const dim3 grid((unsigned)((p.N + 16 * RT - 1) / (16 * RT)), (unsigned)((p.M + 16 * TT - 1) / (16 * TT))), block(64 * kFewWaves);
-  if (src == SRC_MX) hipLaunchKernelGGL((amos_mx_gemm_few<SRC_MX, RT, TT>), grid, block, 0, stream, p);
-  else if (src == SRC_F32) hipLaunchKernelGGL((amos_mx_gemm_few<SRC_F32, RT, TT>), grid, block, 0, stream, p);
-  else if (src == SRC_F16) hipLaunchKernelGGL((amos_mx_gemm_few<SRC_F16, RT, TT>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((amos_mx_gemm_few<SRC_BF16, RT, TT>), grid, block, 0, stream, p);
+template <int SRC, int RT, int TT>
+static int launch_few(const MxGemmParams& p, hipStream_t stream) {
+  constexpr int MAXW = TT == 1 ? 16 : 8;   // (the waves' sums: at most 64 KB)
+  int waves = (p.steps + kTurn - 1) / kTurn;
+  if (waves > MAXW) waves = MAXW;
+  const int64_t gy = ((int64_t)p.M + 16 * TT - 1) / (16 * TT);
+  if (gy > 65535) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d rows and K %d", p.M, p.K);
+  const size_t lds = waves > 1 ? (size_t)waves * RT * TT * 1024 : 0;
+  hipLaunchKernelGGL((amos_mx_gemm_few<SRC, RT, TT, MAXW>), dim3((unsigned)((p.N + 16 * RT - 1) / (16 * RT)), (unsigned)gy),
+                     dim3((unsigned)(64 * waves)), lds, stream, p);
+  return 0;
+}
+
+// Row blocks a workgroup takes.  Every workgroup reads all of its tokens' codes, and what limits it then is the rate of
+// its load instructions; so a grid that one round of the 256 compute units can take is given as few workgroups as
+// that (24 x 10240 x 8192: 1, 2, 3, 4 blocks 23.5, 20.5, 15.8, 16.6 us; 24 x 4096 x 4096: 1, 2, 4 blocks 5.7, 7.1, 9.7 us;
+// 8 x 10240 x 8192: 1, 2, 3 blocks 14.9, 15.7, 11.7 us).  Longer grids: one block a workgroup where the tokens' codes are few
+// (1 x 16384 x 4096: 1, 2, 3, 4 blocks 9.0, 9.0, 11.1, 13.3 us), four where they are not (24 x 28672 x 8192: 2, 4 blocks 39.8, 35.7 us).
+static int few_blocks(int64_t blocks, int tt) {
+  const int64_t rt = (blocks + 255) / 256;
+  return tt == 1 ? (rt <= 3 ? (int)rt : 1) : (rt <= 4 ? (int)rt : 4);
+}
+template <int TT>
+static int pick_few(const MxGemmParams& p, int64_t blocks, hipStream_t stream) {
+  const int rt = few_blocks(blocks, TT);
+  if (rt == 1) return launch_few<SRC_MX, 1, TT>(p, stream);
+  if (rt == 2) return launch_few<SRC_MX, 2, TT>(p, stream);
+  if (rt == 3) return launch_few<SRC_MX, 3, TT>(p, stream);
+  if constexpr (TT > 1) return launch_few<SRC_MX, 4, TT>(p, stream);
+  else return launch_few<SRC_MX, 1, TT>(p, stream);
+}
+template <int SRC>
+static int pick_fused(const MxGemmParams& p, int64_t blocks, hipStream_t stream) {
+  const int rt = few_blocks(blocks, 1);
+  if (rt == 2) return launch_few<SRC, 2, 1>(p, stream);
+  if (rt == 3) return launch_few<SRC, 3, 1>(p, stream);
+  return launch_few<SRC, 1, 1>(p, stream);
 }
 
 // ---- many rows of A -----------------------------------------------------------------------------
 template <int WI, int WJ, int BI, int BJ>
 static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
-  constexpr int lds = 2 * (BI + BJ) * 136;
+  constexpr int lds = 2 * (BI + BJ) * 160;
   void (*const fn)(const MxTileParams) = amos_mx_gemm_tile<WI, WJ, BI, BJ>;
   static std::once_flag once;
   static hipError_t err = hipSuccess;
@@ -167,9 +239,10 @@ static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   t.tiles_j = (p.N + BJ - 1) / BJ;
   t.per_split = (p.steps + 1) / 2;
   t.slices = nullptr;
-  const int es = dense_size(p.out_dtype);
-  t.vec_out = ((uintptr_t)p.c & 15) == 0 && ((int64_t)p.N * es) % 16 == 0;
+  t.vec_out = ((uintptr_t)p.c & 15) == 0 && ((int64_t)p.N * dense_size(p.out_dtype)) % 16 == 0;
+  t.stream_out = (int64_t)p.M * p.N * 4 > (int64_t)32 << 20;
   t.vec_add = p.tail.add && ((uintptr_t)p.tail.add & 15) == 0;   // (N is a multiple of the run then)
+  t.vec_scales = p.steps % 4 == 0 && (((uintptr_t)p.as | (uintptr_t)p.bs) & 15) == 0;
   if ((int64_t)t.tiles_i * t.tiles_j >= (int64_t)1 << 31) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d x %d results", p.M, p.N);
   hipLaunchKernelGGL(fn, dim3((unsigned)(t.tiles_i * t.tiles_j), 1), dim3(64 * WI * WJ), lds, stream, t);
   return 0;
@@ -191,8 +264,11 @@ static int check_desc(const amos_mxfp4_gemm_desc_t* d) {
 
 static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// A's rows are quantised by a launch of their own: codes and scales in the workspace
-static bool quantize_first(const amos_mxfp4_gemm_desc_t* d) { return d->a_dtype != AMOS_MXFP4; }
+// Dense rows of A are quantised by the few-rows kernel itself where every workgroup can afford to read all of them:
+// up to four rows their bytes are fewer than those of the sixteen rows of B that it reads anyway.  More: by a
+// launch of its own, codes and scales in the workspace.
+constexpr int kFusedRows = 4;
+static bool quantize_first(const amos_mxfp4_gemm_desc_t* d) { return d->a_dtype != AMOS_MXFP4 && d->M > kFusedRows; }
 
 static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, const void* A, const void* a_scales, const void* B,
                const void* b_scales, void* C, void* workspace, size_t ws_bytes, hipStream_t stream) {
@@ -224,8 +300,13 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
   p.K = (int)d->K;
   p.steps = (int)(mx_pitch(d->K) / 64);
   p.out_dtype = d->out_dtype;
+  p.vec_out = ((uintptr_t)C & 15) == 0 && d->N % 4 == 0;
   int src = SRC_MX;
-  if (quantize_first(d)) {
+  if (dense && !quantize_first(d)) {
+    p.dense = A;
+    p.dense_vec = ((uintptr_t)A & 15) == 0 && (d->K * dense_size(d->a_dtype)) % 16 == 0;
+    src = d->a_dtype == AMOS_F32 ? SRC_F32 : d->a_dtype == AMOS_F16 ? SRC_F16 : SRC_BF16;
+  } else if (quantize_first(d)) {
     const int64_t code_bytes = round256(d->M * mx_pitch(d->K));
     if (!workspace || ws_bytes < amos_mxfp4_gemm_workspace_bytes(d) || ((uintptr_t)workspace & 255))
       return set_error(AMOS_ERR_WORKSPACE, "4-bit product: %zu bytes of 256-byte aligned workspace wanted for A's codes", amos_mxfp4_gemm_workspace_bytes(d));
@@ -244,19 +325,25 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
     p.a = (const unsigned char*)A;
     p.as = (const unsigned char*)a_scales;
   }
-  // (the tiled kernel's offsets inside a tile have 32 bits)
-  if (d->M > 64 && p.steps < 1 << 18) {
+  // Blocks of 16 rows of B times runs of 16 (up to 16 rows of A) or 32 tokens; few_blocks of them are a workgroup.
+  // Beyond six rounds of the compute units and 32 rows of A the tiled kernel is ahead (384 x 2048 x 4096: 16.2 / 17.6 us; 200 x 4096 x 2048:
+  // 9.8 / 9.2; 64 x 28672 x 8192: 65 / 45; 512 x 1024 x 2048: 6.4 / 9.2); its offsets inside a tile have 32 bits.
+  const int64_t blocks = (d->N + 15) / 16 * (d->M <= 16 ? 1 : (d->M + 31) / 32);
+  if (d->M > 32 && blocks > 6 * 256 && p.steps < 1 << 18) {
     const int64_t big = ((d->M + 255) / 256) * ((d->N + 255) / 256);
     rc = big >= 256 ? launch_tile<4, 2, 256, 256>(p, stream) : launch_tile<2, 4, 128, 128>(p, stream);
-    if (rc) return rc;
-    const hipError_t err = hipGetLastError();
-    if (err != hipSuccess) return set_error(AMOS_ERR_HIP, "launch failed: %s", hipGetErrorString(err));
-    return 0;
+  } else if (src == SRC_F32) {
+    rc = pick_fused<SRC_F32>(p, blocks, stream);
+  } else if (src == SRC_F16) {
+    rc = pick_fused<SRC_F16>(p, blocks, stream);
+  } else if (src == SRC_BF16) {
+    rc = pick_fused<SRC_BF16>(p, blocks, stream);
+  } else if (d->M <= 16) {
+    rc = pick_few<1>(p, blocks, stream);
+  } else {
+    rc = pick_few<2>(p, blocks, stream);
   }
-  if ((d->M + 63) / 64 > 65535) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of more than %d rows", 65535 * 64);
-  if (d->M <= 16) launch_few<1, 1>(p, src, stream);
-  else if (d->M <= 32) launch_few<2, 2>(p, src, stream);
-  else launch_few<2, 4>(p, src, stream);
+  if (rc) return rc;
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return set_error(AMOS_ERR_HIP, "launch failed: %s", hipGetErrorString(err));
   return 0;
@@ -270,7 +357,7 @@ extern "C" {
 
 size_t amos_mxfp4_gemm_workspace_bytes(const amos_mxfp4_gemm_desc_t* desc) {
   if (check_desc(desc)) return 0;
-  if (!quantize_first(desc)) return 0;
+  if (!quantize_first(desc)) return 0;   // (nothing to keep)
   const int64_t pitch = mx_pitch(desc->K);
   return (size_t)(round256(desc->M * pitch) + round256(desc->M * (pitch / 16)));
 }

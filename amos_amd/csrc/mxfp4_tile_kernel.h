@@ -1,9 +1,9 @@
 // Tiled product of two microscaled 4-bit matrices: many rows on both sides.
 //
-// Block tile BI x BJ, K step 256 elements = 128 bytes of every row, two stages in LDS of (BI + BJ) * 136
-// bytes: the codes as rows of eight 16-byte chunks (XOR-swizzled by row, the swizzle applied on the
-// global side), behind them eight scale bytes a row.  Both travel by direct copies (global_load_lds, 16
-// and 4 bytes a lane).  A K step is two matrix instructions deep and runs in four phases (half of
+// Block tile BI x BJ, K step 256 elements = 128 bytes of every row.  LDS holds two stages of codes (rows of
+// eight 16-byte chunks, XOR-swizzled by row, the swizzle applied on the global side) and two spans of
+// scales (32 bytes a row: four K steps).  Both travel by direct copies (global_load_lds, 16 bytes a
+// lane; 4 for scales that are not 16-byte aligned).  A K step is two matrix instructions deep and runs in four phases (half of
 // the wave tile's rows, sub-step); the fragments of a phase are read while the one before multiplies.
 // The one barrier of a step stands in front of its last phase, where all reads of the stage are
 // issued; the copies of the step after next start behind it, spread over three phases.  A fragment is
@@ -25,7 +25,9 @@ struct MxTileParams {
   int tiles_i, tiles_j;
   int per_split;        // K steps of a split (blockIdx.y); its sums go to `slices` + y * M * N, fp32
   float* slices;        // null: not split
+  int vec_scales;       // rows of scales are whole 16-byte pieces from 16-byte aligned memory on
   int vec_out;          // C's rows are whole 16-byte pieces
+  int stream_out;       // an fp32 C larger than the L2s together: written past them (8192^3: 281 -> 270 us)
   int vec_add;          // ... and D's can be read by the same pieces
 };
 
@@ -62,11 +64,12 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   constexpr int TI = BI / (16 * WI), TJ = BJ / (16 * WJ);
   constexpr int HA = TI / 2;
   static_assert(TI % 2 == 0 && TI * WI * 16 == BI && TJ * WJ * 16 == BJ && TJ >= 1, "wave tile");
-  constexpr int OPER = BI * 128, CODES = (BI + BJ) * 128, STAGE = (BI + BJ) * 136;
+  constexpr int OPER = BI * 128, STAGE = (BI + BJ) * 128;        // one stage of codes
+  constexpr int SCALES = 2 * STAGE, SPAN = (BI + BJ) * 32;       // behind both: two spans (four K steps) of scales
   constexpr int QA = BI / 8;
-  constexpr int CH = (BI + BJ) / 8 / NW, SCH = (BI + BJ) / 32 / NW;
-  static_assert(CH >= 1 && CH * NW * 8 == BI + BJ && SCH >= 1 && SCH * NW * 32 == BI + BJ, "copies");
-  constexpr int COPIES = CH + SCH, NS = 2;
+  constexpr int CH = (BI + BJ) / 8 / NW;                         // 1 KB copies of a wave and K step
+  constexpr int SV = (BI + BJ) / 32 / NW, SD = SV;               // copies of scales: a wave and span (16 bytes a lane), a wave and K step (4)
+  static_assert(CH >= 1 && CH * NW * 8 == BI + BJ && SV >= 1 && SV * NW * 32 == BI + BJ, "copies");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const MxGemmParams& p = t.g;
   const int lane = threadIdx.x & 63;
@@ -86,7 +89,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   if (steps > 2 * t.per_split) steps = 2 * t.per_split;
   const int full = steps >> 1, half = steps & 1, KT = full + half;
 
-  unsigned g_off[CH], s_off[SCH];
+  unsigned g_off[CH];
   const int chunk = (lane & 7) ^ (((lane >> 3) ^ (wave & 1)) & 7);   // (NW even: the same for every copy of the wave)
   static_assert(NW % 2 == 0 && QA % 2 == 0, "one swizzle term per wave");
 #pragma unroll
@@ -96,30 +99,54 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     const int r = q < QA ? (bi0 + row < p.M ? row : p.M - 1 - bi0) : (bj0 + row < p.N ? row : p.N - 1 - bj0);
     g_off[u] = (unsigned)r * (unsigned)pitch + chunk * 16;
   }
-#pragma unroll
-  for (int u = 0; u < SCH; ++u) {
-    const int row = (wave + NW * u) * 32 + (lane >> 1);
-    const int r = row < BI ? (bi0 + row < p.M ? row : p.M - 1 - bi0) : (bj0 + row - BI < p.N ? row - BI : p.N - 1 - bj0);
-    s_off[u] = (unsigned)r * (unsigned)spitch + (lane & 1) * 4;
-  }
-  const unsigned back = chunk >= 4 ? 64 : 0, sback = (lane & 1) * 4;   // what a half step's second half steps back
-  // Copy u of step kt (the codes first, then the scales).  As assembly: behind the builtin the compiler lets every
-  // later LDS read wait for all LDS reads before it.  The wait states are those of an address register pair that
-  // a vector instruction may have written (5) and of M0 (1).
+  const unsigned back = chunk >= 4 ? 64 : 0;   // what a half step's second half steps back
+  // Copies as assembly: behind the builtin the compiler lets every later LDS read wait for all LDS reads before it.
+  // The wait states are those of an address register pair that a vector instruction may have written (5) and of M0 (1).
   const unsigned lds0 = (unsigned)(uintptr_t)AMOS_MX_LDS(smem);
   auto issue_copy = [&](int kt, int stage, int u) {
-    const bool h = kt >= full;
-    const unsigned s = lds0 + stage * STAGE;
-    if (u < CH) {
-      const int q = wave + NW * u;
-      const unsigned char* const base = (q < QA ? abase : bbase) + (int64_t)kt * 128;
-      const unsigned off = g_off[u] - (h ? back : 0u);
-      asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(s + q * 1024), "v"(off), "s"(base) : "memory");
+    const int q = wave + NW * u;
+    const unsigned char* const base = (q < QA ? abase : bbase) + (int64_t)kt * 128;
+    const unsigned off = g_off[u] - (kt >= full ? back : 0u);
+    asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + stage * STAGE + q * 1024), "v"(off), "s"(base) : "memory");
+  };
+  // Scales: a row's 32 bytes of four K steps at once (8 bytes a row and step would touch as many memory lines per
+  // step as the codes do).  Bit 3 of the row swaps the two 16-byte halves of its place: sixteen rows on different
+  // banks.  What lies behind a row's end is fetched from its last bytes (and not used).
+  auto scale_row = [&](int row, const unsigned char*& base) -> unsigned {   // row of the tile (A's, then B's) -> row in memory
+    base = row < BI ? asbase : bsbase;
+    return (unsigned)(row < BI ? (bi0 + row < p.M ? row : p.M - 1 - bi0) : (bj0 + row - BI < p.N ? row - BI : p.N - 1 - bj0));
+  };
+  auto scale_vec = [&](int span, int u) {      // 32 rows, two lanes a row
+    const int first = (wave + NW * u) * 32, row = first + (lane >> 1);
+    const int want = span * 32 + ((lane ^ (row >> 3)) & 1) * 16;
+    const unsigned char* base;
+    const unsigned r = scale_row(row, base);
+    const int last = (int)spitch - kt0 * 8 - 16;
+    const unsigned off = r * (unsigned)spitch + (unsigned)(want < last ? want : last);
+    const unsigned char* const sb = first < BI ? asbase : bsbase;
+    asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + SCALES + (span & 1) * SPAN + first * 32), "v"(off), "s"(sb) : "memory");
+  };
+  auto scale_word = [&](int span, int u) {     // 8 rows, eight lanes a row
+    const int first = (wave + NW * u) * 8, row = first + (lane >> 3);
+    const int want = span * 8 + ((lane & 7) ^ (((row >> 3) & 1) << 2));
+    const unsigned char* base;
+    const unsigned r = scale_row(row, base);
+    const int last = p.steps - kt0 * 2 - 1;
+    const unsigned off = r * (unsigned)spitch + (unsigned)(want < last ? want : last) * 4;
+    const unsigned char* const sb = first < BI ? asbase : bsbase;
+    asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds0 + SCALES + (span & 1) * SPAN + first * 32), "v"(off), "s"(sb) : "memory");
+  };
+  // step kt's share of the next span's scales
+  auto issue_scales = [&](int kt) {
+    const int span = (kt >> 2) + 1;
+    if (span * 4 >= KT) return;
+    if (t.vec_scales) {
+      if ((kt & 3) == 0)
+#pragma unroll
+        for (int u = 0; u < SV; ++u) scale_vec(span, u);
     } else {
-      const int q = wave + NW * (u - CH);
-      const unsigned char* const base = (q * 32 < BI ? asbase : bsbase) + (int64_t)kt * 8;
-      const unsigned off = s_off[u - CH] - (h ? sback : 0u);
-      asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(s + CODES + q * 256), "v"(off), "s"(base) : "memory");
+#pragma unroll
+      for (int u = 0; u < SD; ++u) scale_word(span, (kt & 3) * SD + u);
     }
   };
 
@@ -128,7 +155,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   const int frag_row = lane & 15, frag_q = lane >> 4;
   const int arow = wi * TI * 16 + frag_row, brow = wj * TJ * 16 + frag_row;
   const int a_off = mx_lds_offset(arow, 2 * frag_q), b_off = OPER + mx_lds_offset(brow, 2 * frag_q);
-  const int as_off = CODES + arow * 8 + 2 * frag_q, bs_off = CODES + (BI + brow) * 8 + 2 * frag_q;
+  const int swap = ((frag_row >> 3) & 1) * 16;
+  const int as_off = arow * 32 + 2 * frag_q + swap, bs_off = (BI + brow) * 32 + 2 * frag_q + swap;
+  // LDS address of step kt's scale bytes for a row whose place is `off`
+  auto scale_at = [&](int off, int kt) { return smem + SCALES + ((kt >> 2) & 1) * SPAN + (off ^ (((kt >> 1) & 1) * 16)) + (kt & 1) * 8; };
 
   v4f acc[TI][TJ];
 #pragma unroll
@@ -138,26 +168,28 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
 
   mx_v4i af[2][HA], bf[2][TJ];      // A: by half of the wave tile's rows; B: by sub-step
   int ax[TI], bx[TJ], bx_next[TJ];   // scales: a register serves both sub-steps
-  auto read_a = [&](int stage, auto h, auto ks) {
-    const char* s = smem + stage * STAGE;
+  auto read_a = [&](int kt, auto h, auto ks) {
+    const char* s = smem + (kt & 1) * STAGE;
+    const char* x = scale_at(as_off, kt);
 #pragma unroll
     for (int a = 0; a < HA; ++a) {
       af[h][a] = *(const mx_v4i*)(s + (a_off ^ (ks * 16)) + (h * HA + a) * 2048);
-      if (ks == 0) ax[h * HA + a] = *(const unsigned short*)(s + as_off + (h * HA + a) * 128);
+      if (ks == 0) ax[h * HA + a] = *(const unsigned short*)(x + (h * HA + a) * 512);
     }
   };
-  auto read_b = [&](int stage, auto ks, int* x) {
-    const char* s = smem + stage * STAGE;
+  auto read_b = [&](int kt, auto ks, int* to) {
+    const char* s = smem + (kt & 1) * STAGE;
+    const char* x = scale_at(bs_off, kt);
 #pragma unroll
     for (int b = 0; b < TJ; ++b) {
       bf[ks][b] = *(const mx_v4i*)(s + (b_off ^ (ks * 16)) + b * 2048);
-      if (ks == 0) x[b] = *(const unsigned short*)(s + bs_off + b * 128);
+      if (ks == 0) to[b] = *(const unsigned short*)(x + b * 512);
     }
   };
   // One phase: the matrix instructions of half h of sub-step ks, and between them a share of the copies of step kt (a
   // copy keeps its wave from issuing for some 64 cycles: spread out, the matrix core works through them).  The fences
   // keep the compiler from moving the reads in front of a phase down to their use.
-  constexpr int PERG = (COPIES + 3 * TJ - 1) / (3 * TJ);   // copies behind a group of HA instructions: three phases carry them
+  constexpr int SLOTS = 3 * TJ;   // places behind a group of HA instructions in the three phases that carry copies
   auto phase = [&](auto h, auto ks, int part, int kt, int stage) {
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -165,12 +197,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
 #pragma unroll
       for (int a = 0; a < HA; ++a) acc[h * HA + a][b] = mx_mfma<ks>(af[h][a], bf[ks][b], acc[h * HA + a][b], ax[h * HA + a], bx[b]);
       if (part >= 0) {
+        const int slot = part * TJ + b;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int i = 0; i < PERG; ++i) {
-          const int u = (part * TJ + b) * PERG + i;
-          if (u < COPIES) issue_copy(kt, stage, u);
-        }
+        for (int u = slot * CH / SLOTS; u < (slot + 1) * CH / SLOTS; ++u) issue_copy(kt, stage, u);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -178,11 +208,18 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   };
   constexpr std::integral_constant<int, 0> I0{};
   constexpr std::integral_constant<int, 1> I1{};
-  constexpr int FIRST = PERG * TJ < COPIES ? PERG * TJ : COPIES;   // copies of part 0
+  constexpr int FIRST = TJ * CH / SLOTS;   // copies of part 0
 
   // step 0 whole, of step 1 the part that otherwise leaves in the step before
 #pragma unroll
-  for (int u = 0; u < COPIES; ++u) issue_copy(0, 0, u);
+  for (int u = 0; u < CH; ++u) issue_copy(0, 0, u);
+  if (t.vec_scales) {
+#pragma unroll
+    for (int u = 0; u < SV; ++u) scale_vec(0, u);
+  } else {
+#pragma unroll
+    for (int u = 0; u < 4 * SD; ++u) scale_word(0, u);
+  }
 #pragma unroll
   for (int u = 0; u < FIRST; ++u) issue_copy(1 < KT ? 1 : KT - 1, 1, u);
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(FIRST) : "memory");
@@ -191,18 +228,19 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
 
   for (int kt = 0; kt < full; ++kt) {
     const int st = kt & 1, next = kt + 1 < KT ? kt + 1 : KT - 1, after = kt + 2 < KT ? kt + 2 : KT - 1;
-    read_a(st, I1, I0);
+    read_a(kt, I1, I0);
     phase(I0, I0, 1, next, st ^ 1);
-    read_a(st, I0, I1);
-    read_b(st, I1, bx);
+    issue_scales(kt);
+    read_a(kt, I0, I1);
+    read_b(kt, I1, bx);
     phase(I1, I0, 2, next, st ^ 1);
-    read_a(st, I1, I1);
+    read_a(kt, I1, I1);
     phase(I0, I1, -1, 0, 0);
     // all reads of this stage are issued; once they and this wave's copies of the next step are done, meet: behind the
     // barrier the next stage is whole and this one is free
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    read_a(st ^ 1, I0, I0);   // (behind the last step: read and not used)
-    read_b(st ^ 1, I0, bx_next);
+    read_a(kt + 1, I0, I0);   // (behind the last step: read and not used)
+    read_b(kt + 1, I0, bx_next);
     phase(I1, I1, 0, after, st);
 #pragma unroll
     for (int b = 0; b < TJ; ++b) bx[b] = bx_next[b];
@@ -210,16 +248,16 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   if (half) {   // four blocks, one for each lane group
     const char* s = smem + (full & 1) * STAGE;
     const int ah = mx_lds_offset(arow, frag_q), bh = OPER + mx_lds_offset(brow, frag_q);
-    const int axh = CODES + arow * 8 + frag_q, bxh = CODES + (BI + brow) * 8 + frag_q;
+    const char *axh = scale_at(as_off - frag_q, full), *bxh = scale_at(bs_off - frag_q, full);   // (byte q, not 2q)
 #pragma unroll
     for (int b = 0; b < TJ; ++b) {
       bf[0][b] = *(const mx_v4i*)(s + bh + b * 2048);
-      bx[b] = *(const unsigned char*)(s + bxh + b * 128);
+      bx[b] = *(const unsigned char*)(bxh + b * 512);
     }
 #pragma unroll
     for (int a = 0; a < TI; ++a) {
       const mx_v4i f = *(const mx_v4i*)(s + ah + a * 2048);
-      const int x = *(const unsigned char*)(s + axh + a * 128);
+      const int x = *(const unsigned char*)(axh + a * 512);
 #pragma unroll
       for (int b = 0; b < TJ; ++b) acc[a][b] = mx_mfma(f, bf[0][b], acc[a][b], x, bx[b]);
     }
@@ -229,7 +267,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   // a lane; bias and D join there, in fp32, before the one rounding
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");   // (the last copies have landed, all reads are done)
   constexpr int SP = TJ * 16 + 4, SR = HA * 16;
-  static_assert(NW * SR * SP * 4 <= NS * STAGE, "output strip");
+  static_assert(NW * SR * SP * 4 <= SCALES + 2 * SPAN, "output strip");
   float* const strip = (float*)smem + wave * (SR * SP);
   const bool split = t.slices != nullptr;
   void* const out = split ? (void*)(t.slices + (int64_t)blockIdx.y * p.M * p.N) : p.c;
@@ -251,7 +289,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
       for (int x = 0; x < V; ++x) v[x] += e[x];
     }
     if constexpr (V == 4) {
-      DenseVec<TypeF32, 4>::store((float*)out + at, v);
+      if (t.stream_out) DenseVec<TypeF32, 4>::store_streaming((float*)out + at, v);
+      else DenseVec<TypeF32, 4>::store((float*)out + at, v);
     } else {
       if (out_dtype == AMOS_F16) DenseVec<TypeF16, 8>::store((_Float16*)out + at, v);
       else DenseVec<TypeBF16, 8>::store((__bf16*)out + at, v);
