@@ -182,11 +182,5 @@ __device__ __forceinline__ void gn_group_sums(const GnParams& p, const GnSlab& w
   }
   __syncthreads();
 }
-template <int VEC>
-__device__ __forceinline__ void gn_store_any(void* p, int64_t at, int dtype, const float* v) {
-  if (dtype == AMOS_F32) DenseVec<TypeF32, VEC>::store((float*)p + at, v);
-  else if (dtype == AMOS_F16) DenseVec<TypeF16, VEC>::store((_Float16*)p + at, v);
-  else DenseVec<TypeBF16, VEC>::store((__bf16*)p + at, v);
-}
 
 }  // namespace amos

@@ -397,11 +397,10 @@ static int run_gradient(const amos_group_norm_desc_t* d, const void* dy, const v
                         const float* rstd, void* dx, float* dweight, float* dbias, void* workspace, size_t ws_bytes, hipStream_t stream) {
   GnParams p;
   GnPlan plan;
-  bool wide;
-  int rc = gn_check(d, {dy, x, dx}, weight, bias, p, wide);
+  int rc = gn_check(d, {dy, x, dx}, weight, bias, p);
   if (rc) return rc;
   if (!mean || !rstd) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
-  rc = gn_choose(d, true, wide, p, plan);
+  rc = gn_choose(d, true, p, plan);
   if (rc == 0) rc = gn_workspace(plan, p, workspace, ws_bytes);
   if (rc) return rc;
   p.x = x;

@@ -247,7 +247,7 @@ __global__ __launch_bounds__(1024) void amos_gn_held(const GnParams p) {
     V::widen(raw[r], v);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) v[i] = gn_act((v[i] - mean[UNI ? 0 : i]) * gamma[i] + beta[i], p.act);
-    gn_store_any<VEC>(p.out, w.n * p.image + w.c + (int64_t)q * p.pixel, p.y_dtype, v);
+    store_run_any<VEC>(p.out, w.n * p.image + w.c + (int64_t)q * p.pixel, p.y_dtype, v);
   }
 }
 
@@ -289,9 +289,8 @@ static int run_forward(const amos_group_norm_desc_t* d, const void* x, const voi
                        void* workspace, size_t ws_bytes, hipStream_t stream) {
   GnParams p;
   GnPlan plan;
-  bool wide;
-  int rc = gn_check(d, {x, y}, weight, bias, p, wide);
-  if (rc == 0) rc = gn_choose(d, false, wide, p, plan);
+  int rc = gn_check(d, {x, y}, weight, bias, p);
+  if (rc == 0) rc = gn_choose(d, false, p, plan);
   if (rc == 0) rc = gn_workspace(plan, p, workspace, ws_bytes);
   if (rc) return rc;
   p.x = x;

@@ -105,18 +105,16 @@ inline int gn_plan_tiles(const amos_group_norm_desc_t* d, bool gradient, int vec
   return 0;
 }
 
-// `wide`: all tensors are 16-byte aligned
-inline int gn_choose(const amos_group_norm_desc_t* d, bool gradient, bool wide, GnParams& p, GnPlan& plan) {
+inline int gn_choose(const amos_group_norm_desc_t* d, bool gradient, GnParams& p, GnPlan& plan) {
   const int vec = d->x_dtype == AMOS_F32 || d->y_dtype == AMOS_F32 ? 4 : 8;   // 16 bytes of the wider type
-  if (wide && d->C % vec == 0 && gn_plan_held(d, gradient, vec, p, plan)) return 0;
-  if (!(wide && d->C % 8 == 0) && gn_plan_held(d, gradient, 1, p, plan)) return 0;
-  int rc = wide ? gn_plan_tiles(d, gradient, vec, p, plan) : 1;
+  const bool divides = d->C % vec == 0;
+  if (gn_plan_held(d, gradient, divides ? vec : 1, p, plan)) return 0;
+  int rc = divides ? gn_plan_tiles(d, gradient, vec, p, plan) : 1;
   if (rc == 1) rc = gn_plan_tiles(d, gradient, 1, p, plan);
   return rc;
 }
 
-inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<const void*> tensors, const void* weight, const void* bias, GnParams& p,
-                    bool& wide) {
+inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<const void*> tensors, const void* weight, const void* bias, GnParams& p) {
   if (!d) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
   for (const void* t : tensors)
     if (!t) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
@@ -149,27 +147,17 @@ inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<const
   p.weight = weight;
   p.bias = bias;
   const int es = dense_size(d->x_dtype) < dense_size(d->y_dtype) ? dense_size(d->x_dtype) : dense_size(d->y_dtype);
-  wide = true;
-  for (const void* t : tensors) {
+  for (const void* t : tensors)
     if ((uintptr_t)t & (es - 1)) return set_error(AMOS_ERR_BAD_ARG, "group norm: misaligned tensor");
-    wide = wide && ((uintptr_t)t & 15) == 0;
-  }
   return 0;
 }
 
 inline size_t gn_plan_bytes(const GnPlan& plan) { return (size_t)((plan.part_floats + 1) / 2 * 2 + plan.cpart_floats) * sizeof(float); }
-// enough for whatever kernel the pointers' alignment leads to
 inline size_t gn_workspace_bytes(const amos_group_norm_desc_t* d, bool gradient) {
   GnParams p;
   GnPlan plan;
-  bool wide;
-  if (gn_check(d, {}, nullptr, nullptr, p, wide)) return 0;
-  size_t need = 0;
-  for (const bool aligned : {true, false}) {
-    if (gn_choose(d, gradient, aligned, p, plan)) return 0;
-    need = gn_plan_bytes(plan) > need ? gn_plan_bytes(plan) : need;
-  }
-  return need;
+  if (gn_check(d, {}, nullptr, nullptr, p) || gn_choose(d, gradient, p, plan)) return 0;
+  return gn_plan_bytes(plan);
 }
 
 inline int gn_workspace(const GnPlan& plan, GnParams& p, void* workspace, size_t ws_bytes) {

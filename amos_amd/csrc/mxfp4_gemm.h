@@ -32,8 +32,6 @@ struct MxGemmParams {
   int M, N, K;
   int steps;               // pitch / 64: steps of K = 128
   int out_dtype;
-  int dense_vec;           // rows of `dense` are 16-byte aligned
-  int vec_out;             // rows of C are whole runs of four elements from 16-byte aligned memory on
   MxTail tail;
 };
 

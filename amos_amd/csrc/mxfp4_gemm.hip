@@ -29,7 +29,7 @@ template <class T>
 __device__ __forceinline__ void mx_quantize_fragment(const MxGemmParams& p, int64_t m, int64_t k, mx_v4i& codes, int& scale) {
   const typename T::raw_t* const x = (const typename T::raw_t*)p.dense + m * p.K + k;
   float v[32];
-  if (p.dense_vec && k + 32 <= p.K) {
+  if (k + 32 <= p.K) {
     constexpr int N = 16 / T::ES;
     typename DenseVec<T, N>::vec_t raw[32 / N];
 #pragma unroll
@@ -145,15 +145,8 @@ __global__ __launch_bounds__(64 * MAXW) void amos_mx_gemm_few(const MxGemmParams
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] += e[k];
       }
-      if (p.vec_out) {
-        const float w[4] = {v[0], v[1], v[2], v[3]};
-        if (p.out_dtype == AMOS_F32) DenseVec<TypeF32, 4>::store((float*)p.c + at, w);
-        else if (p.out_dtype == AMOS_F16) DenseVec<TypeF16, 4>::store((_Float16*)p.c + at, w);
-        else DenseVec<TypeBF16, 4>::store((__bf16*)p.c + at, w);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) store_any(p.c, at + k, p.out_dtype, v[k]);
-      }
+      const float w[4] = {v[0], v[1], v[2], v[3]};
+      store_run_any<4>(p.c, at, p.out_dtype, w);
     } else {
       for (int k = 0; k < 4 && n + k < p.N; ++k) store_any(p.c, at + k, p.out_dtype, mx_tail(p.tail, v[k], m, n + k, p.N));
     }
@@ -239,9 +232,7 @@ static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   t.tiles_j = (p.N + BJ - 1) / BJ;
   t.per_split = (p.steps + 1) / 2;
   t.slices = nullptr;
-  t.vec_out = ((uintptr_t)p.c & 15) == 0 && ((int64_t)p.N * dense_size(p.out_dtype)) % 16 == 0;
   t.stream_out = (int64_t)p.M * p.N * 4 > (int64_t)32 << 20;
-  t.vec_add = p.tail.add && ((uintptr_t)p.tail.add & 15) == 0;   // (N is a multiple of the run then)
   t.vec_scales = p.steps % 4 == 0 && (((uintptr_t)p.as | (uintptr_t)p.bs) & 15) == 0;
   if ((int64_t)t.tiles_i * t.tiles_j >= (int64_t)1 << 31) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d x %d results", p.M, p.N);
   hipLaunchKernelGGL(fn, dim3((unsigned)(t.tiles_i * t.tiles_j), 1), dim3(64 * WI * WJ), lds, stream, t);
@@ -300,11 +291,9 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
   p.K = (int)d->K;
   p.steps = (int)(mx_pitch(d->K) / 64);
   p.out_dtype = d->out_dtype;
-  p.vec_out = ((uintptr_t)C & 15) == 0 && d->N % 4 == 0;
   int src = SRC_MX;
   if (dense && !quantize_first(d)) {
     p.dense = A;
-    p.dense_vec = ((uintptr_t)A & 15) == 0 && (d->K * dense_size(d->a_dtype)) % 16 == 0;
     src = d->a_dtype == AMOS_F32 ? SRC_F32 : d->a_dtype == AMOS_F16 ? SRC_F16 : SRC_BF16;
   } else if (quantize_first(d)) {
     const int64_t code_bytes = round256(d->M * mx_pitch(d->K));

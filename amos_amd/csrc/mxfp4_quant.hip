@@ -22,8 +22,7 @@ struct QuantParams {
 
 // Eight elements a lane (16 bytes of a 16-bit type), four neighbouring lanes a block: the block's
 // maximum meets over the quad (two DPP steps), the lane's eight codes are one 32-bit store.
-// VEC: rows and their starts are 16-byte aligned and a lane's eight elements are all there.
-template <class T, bool VEC>
+template <class T>
 __global__ __launch_bounds__(256) void amos_mx_quantize_rows(const QuantParams p) {
   const int unit = blockIdx.x * 256 + threadIdx.x;
   if (unit >= p.units) return;   // (units are a multiple of 16: a quad stays or leaves whole)
@@ -32,7 +31,7 @@ __global__ __launch_bounds__(256) void amos_mx_quantize_rows(const QuantParams p
   const int64_t col = (int64_t)piece * 8;
   const typename T::raw_t* const x = (const typename T::raw_t*)p.x + row * p.ld + col;
   float v[8];
-  if (VEC && col + 8 <= p.cols) {
+  if (col + 8 <= p.cols) {
     if constexpr (T::ES == 2) {
       DenseVec<T, 8>::load(x, v);
     } else {
@@ -107,7 +106,7 @@ __global__ __launch_bounds__(512) void amos_mx_quantize_columns(const QuantParam
   }
 }
 
-template <class T, bool VEC>
+template <class T>
 __global__ __launch_bounds__(256) void amos_mx_dequantize(const QuantParams p) {
   const int unit = blockIdx.x * 256 + threadIdx.x;
   if (unit >= p.units) return;
@@ -119,7 +118,7 @@ __global__ __launch_bounds__(256) void amos_mx_dequantize(const QuantParams p) {
   float v[8];
   mx_decode8(c, s, v);
   typename T::raw_t* const x = (typename T::raw_t*)p.x + row * p.ld + col;
-  if (VEC && col + 8 <= p.cols) {
+  if (col + 8 <= p.cols) {
     if constexpr (T::ES == 2) {
       DenseVec<T, 8>::store(x, v);
     } else {
@@ -134,15 +133,10 @@ __global__ __launch_bounds__(256) void amos_mx_dequantize(const QuantParams p) {
 }
 
 template <class T>
-static void launch_rows(const QuantParams& p, bool vec, bool back, hipStream_t stream) {
+static void launch_rows(const QuantParams& p, bool back, hipStream_t stream) {
   const dim3 grid((unsigned)((p.units + 255) / 256)), block(256);
-  if (back) {
-    if (vec) hipLaunchKernelGGL((amos_mx_dequantize<T, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((amos_mx_dequantize<T, false>), grid, block, 0, stream, p);
-  } else {
-    if (vec) hipLaunchKernelGGL((amos_mx_quantize_rows<T, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((amos_mx_quantize_rows<T, false>), grid, block, 0, stream, p);
-  }
+  if (back) hipLaunchKernelGGL((amos_mx_dequantize<T>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((amos_mx_quantize_rows<T>), grid, block, 0, stream, p);
 }
 template <class T>
 static void launch_columns(const QuantParams& p, unsigned gy, hipStream_t stream) {
@@ -170,7 +164,6 @@ static int run_rows(const amos_mxfp4_desc_t* d, const void* x, void* codes, void
   p.pitch = mx_pitch(d->cols);
   const int64_t per_row = back ? (d->cols + 7) / 8 : p.pitch / 4;
   p.per_row = make_fast_div((uint32_t)per_row);
-  const bool vec = ((uintptr_t)x & 15) == 0 && (d->cols * es) % 16 == 0;
   const int64_t most = ((int64_t)1 << 30) / per_row;   // (per_row < 2^28)
   for (int64_t r = 0; r < d->rows; r += most) {
     p.rows = d->rows - r < most ? d->rows - r : most;
@@ -178,9 +171,9 @@ static int run_rows(const amos_mxfp4_desc_t* d, const void* x, void* codes, void
     p.x = (const char*)x + r * p.ld * es;
     p.codes = (unsigned char*)codes + r * p.pitch;
     p.scales = (unsigned char*)scales + r * (p.pitch / 16);
-    if (d->dtype == AMOS_F32) launch_rows<TypeF32>(p, vec, back, stream);
-    else if (d->dtype == AMOS_F16) launch_rows<TypeF16>(p, vec, back, stream);
-    else launch_rows<TypeBF16>(p, vec, back, stream);
+    if (d->dtype == AMOS_F32) launch_rows<TypeF32>(p, back, stream);
+    else if (d->dtype == AMOS_F16) launch_rows<TypeF16>(p, back, stream);
+    else launch_rows<TypeBF16>(p, back, stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(AMOS_ERR_HIP, "launch failed: %s", hipGetErrorString(e));
   }

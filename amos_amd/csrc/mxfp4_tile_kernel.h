@@ -26,9 +26,7 @@ struct MxTileParams {
   int per_split;        // K steps of a split (blockIdx.y); its sums go to `slices` + y * M * N, fp32
   float* slices;        // null: not split
   int vec_scales;       // rows of scales are whole 16-byte pieces from 16-byte aligned memory on
-  int vec_out;          // C's rows are whole 16-byte pieces
   int stream_out;       // an fp32 C larger than the L2s together: written past them (8192^3: 281 -> 270 us)
-  int vec_add;          // ... and D's can be read by the same pieces
 };
 
 // LDS place of a row's 16-byte chunk.  The swizzle goes by the row inside its block of 16, so that the fragments of
@@ -39,24 +37,6 @@ __device__ __forceinline__ int mx_lds_offset(int row, int chunk) {
 }
 
 #define AMOS_MX_LDS(p) ((__attribute__((address_space(3))) void*)(p))
-
-// V consecutive values of a dense tensor; `whole`: they are aligned to V elements (or 16 bytes)
-template <int V>
-__device__ __forceinline__ void mx_load_run(const void* p, int64_t at, int dtype, int whole, float* v) {
-  if (whole) {
-    if (dtype == AMOS_F32) {
-#pragma unroll
-      for (int i = 0; i < V; i += 4) DenseVec<TypeF32, 4>::load((const float*)p + at + i, v + i);
-    } else if (dtype == AMOS_F16) {
-      DenseVec<TypeF16, V>::load((const _Float16*)p + at, v);
-    } else {
-      DenseVec<TypeBF16, V>::load((const __bf16*)p + at, v);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = load_any(p, at + i, dtype);
-  }
-}
 
 template <int WI, int WJ, int BI, int BJ>
 __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTileParams t) {
@@ -273,27 +253,41 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   void* const out = split ? (void*)(t.slices + (int64_t)blockIdx.y * p.M * p.N) : p.c;
   const int out_dtype = split ? (int)AMOS_F32 : p.out_dtype;
   const int wj0 = bj0 + wj * TJ * 16;
+  const bool bias = !split && p.tail.bias, add = !split && p.tail.add;
   // V neighbouring results of a lane
-  auto emit = [&](int i, int j, float* v, auto width) {
+  auto emit = [&](int i, int j, const float* from, auto width) {
     constexpr int V = decltype(width)::value;
+    float v[V], e[V];
+#pragma unroll
+    for (int x = 0; x < V; x += 4) {
+      const v4f w = *(const v4f*)(from + x);
+#pragma unroll
+      for (int y = 0; y < 4; ++y) v[x + y] = w[y];
+    }
     const int64_t at = (int64_t)i * p.N + j;
-    float e[V];
-    if (!split && p.tail.bias) {
-      mx_load_run<V>(p.tail.bias, j, p.tail.bias_dtype, 0, e);
+    if (i >= p.M || j >= p.N) return;
+    if (j + V <= p.N) {
+      if (bias) {
+        load_run_any<V>(p.tail.bias, j, p.tail.bias_dtype, 0.f, e);
 #pragma unroll
-      for (int x = 0; x < V; ++x) v[x] += e[x];
-    }
-    if (!split && p.tail.add) {
-      mx_load_run<V>(p.tail.add, at, p.tail.add_dtype, t.vec_add, e);
+        for (int x = 0; x < V; ++x) v[x] += e[x];
+      }
+      if (add) {
+        load_run_any<V>(p.tail.add, at, p.tail.add_dtype, 0.f, e);
 #pragma unroll
-      for (int x = 0; x < V; ++x) v[x] += e[x];
-    }
-    if constexpr (V == 4) {
-      if (t.stream_out) DenseVec<TypeF32, 4>::store_streaming((float*)out + at, v);
-      else DenseVec<TypeF32, 4>::store((float*)out + at, v);
+        for (int x = 0; x < V; ++x) v[x] += e[x];
+      }
+      if constexpr (V == 4) {
+        if (t.stream_out) DenseVec<TypeF32, 4>::store_streaming((float*)out + at, v);
+        else DenseVec<TypeF32, 4>::store((float*)out + at, v);
+      } else {
+        if (out_dtype == AMOS_F16) DenseVec<TypeF16, 8>::store((_Float16*)out + at, v);
+        else DenseVec<TypeBF16, 8>::store((__bf16*)out + at, v);
+      }
     } else {
-      if (out_dtype == AMOS_F16) DenseVec<TypeF16, 8>::store((_Float16*)out + at, v);
-      else DenseVec<TypeBF16, 8>::store((__bf16*)out + at, v);
+#pragma unroll
+      for (int x = 0; x < V; ++x)
+        if (j + x < p.N) store_any(out, at + x, out_dtype, split ? v[x] : mx_tail(p.tail, v[x], i, j + x, p.N));
     }
   };
   auto store_half = [&](int h) {
@@ -305,35 +299,20 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
         for (int r = 0; r < 4; ++r) strip[(a * 16 + 4 * frag_q + r) * SP + b * 16 + frag_row] = acc[h * HA + a][b][r];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const int i0 = bi0 + (wi * TI + h * HA) * 16;
-    if (t.vec_out && out_dtype == AMOS_F32) {
+    if (out_dtype == AMOS_F32) {
       constexpr int LPR = TJ * 4, RPI = 64 / LPR;
 #pragma unroll 2
       for (int n = 0; n < SR / RPI; ++n) {
         const int row = n * RPI + lane / LPR, col = (lane % LPR) * 4;
-        float v[4];
-        DenseVec<TypeF32, 4>::load(strip + row * SP + col, v);
-        if (i0 + row < p.M && wj0 + col < p.N) emit(i0 + row, wj0 + col, v, std::integral_constant<int, 4>{});
+        emit(i0 + row, wj0 + col, strip + row * SP + col, std::integral_constant<int, 4>{});
       }
-    } else if (t.vec_out) {
+    } else {
       constexpr int LPR = TJ * 2, RPI = 64 / LPR;
       static_assert(SR % RPI == 0, "strip rows");
 #pragma unroll 2
       for (int n = 0; n < SR / RPI; ++n) {
         const int row = n * RPI + lane / LPR, col = (lane % LPR) * 8;
-        float v[8];
-        DenseVec<TypeF32, 4>::load(strip + row * SP + col, v);
-        DenseVec<TypeF32, 4>::load(strip + row * SP + col + 4, v + 4);
-        if (i0 + row < p.M && wj0 + col < p.N) emit(i0 + row, wj0 + col, v, std::integral_constant<int, 8>{});
-      }
-    } else {
-      for (int e = lane; e < SR * TJ * 16; e += 64) {
-        const int row = e / (TJ * 16), col = e % (TJ * 16);
-        const int i = i0 + row, j = wj0 + col;
-        if (i < p.M && j < p.N) {
-          float v = strip[row * SP + col];
-          if (!split) v = mx_tail(p.tail, v, i, j, p.N);
-          store_any(out, (int64_t)i * p.N + j, out_dtype, v);
-        }
+        emit(i0 + row, wj0 + col, strip + row * SP + col, std::integral_constant<int, 8>{});
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the strip is read before it is written again)
