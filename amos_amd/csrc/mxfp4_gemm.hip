@@ -185,35 +185,25 @@ static int launch_few(const MxGemmParams& p, hipStream_t stream) {
 
 // Row blocks a workgroup takes.  Every workgroup reads all of its tokens' codes, and what limits it then is the rate of
 // its load instructions; so a grid that one round of the 256 compute units can take is given as few workgroups as
-// that (24 x 10240 x 8192: 1, 2, 3, 4 blocks 23.5, 20.5, 15.8, 16.6 us; 24 x 4096 x 4096: 1, 2, 4 blocks 5.7, 7.1, 9.7 us;
-// 8 x 10240 x 8192: 1, 2, 3 blocks 14.9, 15.7, 11.7 us).  Longer grids: one block a workgroup where the tokens' codes are few
-// (1 x 16384 x 4096: 1, 2, 3, 4 blocks 9.0, 9.0, 11.1, 13.3 us), four where they are not (24 x 28672 x 8192: 2, 4 blocks 39.8, 35.7 us).
-static int few_blocks(int64_t blocks, int tt) {
+// that (24 x 4096 x 4096: 1, 2 blocks 5.7, 7.1 us; 32 x 8192 x 2048: 5.8, 4.9 us; 8 x 10240 x 8192: 1, 2, 3 blocks 14.9, 15.7, 11.7 us),
+// longer ones one block a workgroup (1 x 16384 x 4096: 1, 2, 3 blocks 9.0, 9.0, 11.1 us).
+static int few_blocks(int64_t blocks) {
   const int64_t rt = (blocks + 255) / 256;
-  return tt == 1 ? (rt <= 3 ? (int)rt : 1) : (rt <= 4 ? (int)rt : 4);
-}
-template <int TT>
-static int pick_few(const MxGemmParams& p, int64_t blocks, hipStream_t stream) {
-  const int rt = few_blocks(blocks, TT);
-  if (rt == 1) return launch_few<SRC_MX, 1, TT>(p, stream);
-  if (rt == 2) return launch_few<SRC_MX, 2, TT>(p, stream);
-  if (rt == 3) return launch_few<SRC_MX, 3, TT>(p, stream);
-  if constexpr (TT > 1) return launch_few<SRC_MX, 4, TT>(p, stream);
-  else return launch_few<SRC_MX, 1, TT>(p, stream);
+  return rt <= 3 ? (int)rt : 1;
 }
 template <int SRC>
 static int pick_fused(const MxGemmParams& p, int64_t blocks, hipStream_t stream) {
-  const int rt = few_blocks(blocks, 1);
+  const int rt = few_blocks(blocks);
   if (rt == 2) return launch_few<SRC, 2, 1>(p, stream);
   if (rt == 3) return launch_few<SRC, 3, 1>(p, stream);
   return launch_few<SRC, 1, 1>(p, stream);
 }
 
 // ---- many rows of A -----------------------------------------------------------------------------
-template <int WI, int WJ, int BI, int BJ>
+template <int WI, int WJ, int BI, int BJ, int NS>
 static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
-  constexpr int lds = 2 * (BI + BJ) * 160;
-  void (*const fn)(const MxTileParams) = amos_mx_gemm_tile<WI, WJ, BI, BJ>;
+  constexpr int lds = (BI + BJ) * (NS * 128 + 64);
+  void (*const fn)(const MxTileParams) = amos_mx_gemm_tile<WI, WJ, BI, BJ, NS>;
   static std::once_flag once;
   static hipError_t err = hipSuccess;
   static int spilled = 0;
@@ -237,6 +227,19 @@ static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   if ((int64_t)t.tiles_i * t.tiles_j >= (int64_t)1 << 31) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d x %d results", p.M, p.N);
   hipLaunchKernelGGL(fn, dim3((unsigned)(t.tiles_i * t.tiles_j), 1), dim3(64 * WI * WJ), lds, stream, t);
   return 0;
+}
+
+// The tile by how many there are: 64x64 (four waves, four stages, two workgroups a compute unit) while one round takes
+// them or one side has no more rows (2048 x 1024 x 4096: 12.7 us, 128x128 16.4; 4096 x 1024 x 2048, 1024 of them: 15.0 / 11.7);
+// 128x128 in one round with four waves and three stages (4096 x 1024 x 2048: 11.7 us, eight waves 11.8; 1024 x 4096 x 4096:
+// 17.8 / 19.2), beyond that with eight waves and two workgroups a compute unit (4096 x 2048 x 1024: 12.1 us, four waves 13.4);
+// 256x256 from a full round on (4096 x 4096 x 1024: 17.1 us, 128x128 19.9).
+static int pick_tile(const MxGemmParams& p, hipStream_t stream) {
+  const auto tiles = [&](int64_t e) { return (p.M + e - 1) / e * ((p.N + e - 1) / e); };
+  if (tiles(64) <= 512 || p.M <= 64 || p.N <= 64) return launch_tile<2, 2, 64, 64, 4>(p, stream);
+  if (tiles(128) <= 256) return launch_tile<2, 2, 128, 128, 3>(p, stream);
+  if (tiles(256) < 256) return launch_tile<2, 4, 128, 128, 2>(p, stream);
+  return launch_tile<4, 2, 256, 256, 2>(p, stream);
 }
 
 int mx_quantize(const amos_mxfp4_desc_t* d, const void* x, void* codes, void* scales, hipStream_t stream);
@@ -314,23 +317,24 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
     p.a = (const unsigned char*)A;
     p.as = (const unsigned char*)a_scales;
   }
-  // Blocks of 16 rows of B times runs of 16 (up to 16 rows of A) or 32 tokens; few_blocks of them are a workgroup.
-  // Beyond six rounds of the compute units and 32 rows of A the tiled kernel is ahead (384 x 2048 x 4096: 16.2 / 17.6 us; 200 x 4096 x 2048:
-  // 9.8 / 9.2; 64 x 28672 x 8192: 65 / 45; 512 x 1024 x 2048: 6.4 / 9.2); its offsets inside a tile have 32 bits.
+  // Blocks of 16 rows of B times runs of 16 (up to 16 rows of A) or 32 tokens.  Above 16 rows the few-rows kernel is ahead
+  // while they are at most two rounds of the compute units (512 x 512 x 4096: 7.6 us, 64x64 tiles 9.0; 64 x 4096 x 4096: 7.6 / 8.9;
+  // 100 x 4096 x 4096, four rounds: 10.6 / 8.9); the tiled kernels' offsets inside a tile have 32 bits.
   const int64_t blocks = (d->N + 15) / 16 * (d->M <= 16 ? 1 : (d->M + 31) / 32);
-  if (d->M > 32 && blocks > 6 * 256 && p.steps < 1 << 18) {
-    const int64_t big = ((d->M + 255) / 256) * ((d->N + 255) / 256);
-    rc = big >= 256 ? launch_tile<4, 2, 256, 256>(p, stream) : launch_tile<2, 4, 128, 128>(p, stream);
-  } else if (src == SRC_F32) {
+  if (src == SRC_F32) {
     rc = pick_fused<SRC_F32>(p, blocks, stream);
   } else if (src == SRC_F16) {
     rc = pick_fused<SRC_F16>(p, blocks, stream);
   } else if (src == SRC_BF16) {
     rc = pick_fused<SRC_BF16>(p, blocks, stream);
   } else if (d->M <= 16) {
-    rc = pick_few<1>(p, blocks, stream);
+    rc = pick_fused<SRC_MX>(p, blocks, stream);
+  } else if (blocks <= 256 || p.steps >= 1 << 18) {
+    rc = launch_few<SRC_MX, 1, 2>(p, stream);
+  } else if (blocks <= 512) {
+    rc = launch_few<SRC_MX, 2, 2>(p, stream);
   } else {
-    rc = pick_few<2>(p, blocks, stream);
+    rc = pick_tile(p, stream);
   }
   if (rc) return rc;
   const hipError_t err = hipGetLastError();

@@ -1,12 +1,12 @@
 // Tiled product of two microscaled 4-bit matrices: many rows on both sides.
 //
-// Block tile BI x BJ, K step 256 elements = 128 bytes of every row.  LDS holds two stages of codes (rows of
+// Block tile BI x BJ, K step 256 elements = 128 bytes of every row.  LDS holds NS stages of codes (rows of
 // eight 16-byte chunks, XOR-swizzled by row, the swizzle applied on the global side) and two spans of
 // scales (32 bytes a row: four K steps).  Both travel by direct copies (global_load_lds, 16 bytes a
 // lane; 4 for scales that are not 16-byte aligned).  A K step is two matrix instructions deep and runs in four phases (half of
 // the wave tile's rows, sub-step); the fragments of a phase are read while the one before multiplies.
 // The one barrier of a step stands in front of its last phase, where all reads of the stage are
-// issued; the copies of the step after next start behind it, spread over three phases.  A fragment is
+// issued; the copies of the step NS later start behind it, spread over three phases.  A fragment is
 // one 16-byte LDS read; its block's scale is a byte of a register that a 2-byte read fills for both
 // sub-steps and that the matrix instruction takes as it is: no instruction touches a scale.
 // Rows past M / N repeat the last one (their sums are not stored).  K is padded to 128 by the format; an
@@ -38,17 +38,17 @@ __device__ __forceinline__ int mx_lds_offset(int row, int chunk) {
 
 #define AMOS_MX_LDS(p) ((__attribute__((address_space(3))) void*)(p))
 
-template <int WI, int WJ, int BI, int BJ>
+template <int WI, int WJ, int BI, int BJ, int NS>
 __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTileParams t) {
   constexpr int NW = WI * WJ;
   constexpr int TI = BI / (16 * WI), TJ = BJ / (16 * WJ);
   constexpr int HA = TI / 2;
   static_assert(TI % 2 == 0 && TI * WI * 16 == BI && TJ * WJ * 16 == BJ && TJ >= 1, "wave tile");
   constexpr int OPER = BI * 128, STAGE = (BI + BJ) * 128;        // one stage of codes
-  constexpr int SCALES = 2 * STAGE, SPAN = (BI + BJ) * 32;       // behind both: two spans (four K steps) of scales
+  constexpr int SCALES = NS * STAGE, SPAN = (BI + BJ) * 32;      // behind them: two spans (four K steps) of scales
   constexpr int QA = BI / 8;
   constexpr int CH = (BI + BJ) / 8 / NW;                         // 1 KB copies of a wave and K step
-  constexpr int SV = (BI + BJ) / 32 / NW, SD = SV;               // copies of scales: a wave and span (16 bytes a lane), a wave and K step (4)
+  constexpr int SV = (BI + BJ) / 32 / NW, SW = 4 * SV;           // copies of scales of a wave and span: 16 bytes a lane, 4 bytes
   static_assert(CH >= 1 && CH * NW * 8 == BI + BJ && SV >= 1 && SV * NW * 32 == BI + BJ, "copies");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const MxGemmParams& p = t.g;
@@ -116,17 +116,18 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     const unsigned char* const sb = first < BI ? asbase : bsbase;
     asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds0 + SCALES + (span & 1) * SPAN + first * 32), "v"(off), "s"(sb) : "memory");
   };
-  // step kt's share of the next span's scales
+  // step kt's share of the next span's scales (in the first two steps of a span: what follows them until their use is
+  // more than the waits below leave in flight)
   auto issue_scales = [&](int kt) {
     const int span = (kt >> 2) + 1;
-    if (span * 4 >= KT) return;
+    if (span * 4 >= KT || (kt & 2)) return;
     if (t.vec_scales) {
-      if ((kt & 3) == 0)
+      if ((kt & 1) == 0)
 #pragma unroll
         for (int u = 0; u < SV; ++u) scale_vec(span, u);
     } else {
 #pragma unroll
-      for (int u = 0; u < SD; ++u) scale_word(span, (kt & 3) * SD + u);
+      for (int u = 0; u < SW / 2; ++u) scale_word(span, (kt & 1) * (SW / 2) + u);
     }
   };
 
@@ -148,8 +149,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
 
   mx_v4i af[2][HA], bf[2][TJ];      // A: by half of the wave tile's rows; B: by sub-step
   int ax[TI], bx[TJ], bx_next[TJ];   // scales: a register serves both sub-steps
-  auto read_a = [&](int kt, auto h, auto ks) {
-    const char* s = smem + (kt & 1) * STAGE;
+  auto read_a = [&](int kt, int stage, auto h, auto ks) {
+    const char* s = smem + stage * STAGE;
     const char* x = scale_at(as_off, kt);
 #pragma unroll
     for (int a = 0; a < HA; ++a) {
@@ -157,8 +158,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
       if (ks == 0) ax[h * HA + a] = *(const unsigned short*)(x + (h * HA + a) * 512);
     }
   };
-  auto read_b = [&](int kt, auto ks, int* to) {
-    const char* s = smem + (kt & 1) * STAGE;
+  auto read_b = [&](int kt, int stage, auto ks, int* to) {
+    const char* s = smem + stage * STAGE;
     const char* x = scale_at(bs_off, kt);
 #pragma unroll
     for (int b = 0; b < TJ; ++b) {
@@ -190,43 +191,54 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   constexpr std::integral_constant<int, 1> I1{};
   constexpr int FIRST = TJ * CH / SLOTS;   // copies of part 0
 
-  // step 0 whole, of step 1 the part that otherwise leaves in the step before
+  // the first NS - 1 steps whole, of the next one the part that otherwise leaves in the step before
 #pragma unroll
-  for (int u = 0; u < CH; ++u) issue_copy(0, 0, u);
-  if (t.vec_scales) {
+  for (int s = 0; s < NS - 1; ++s) {
 #pragma unroll
-    for (int u = 0; u < SV; ++u) scale_vec(0, u);
-  } else {
+    for (int u = 0; u < CH; ++u) issue_copy(s < KT ? s : KT - 1, s, u);
+    if (s == 0) {
+      if (t.vec_scales) {
 #pragma unroll
-    for (int u = 0; u < 4 * SD; ++u) scale_word(0, u);
+        for (int u = 0; u < SV; ++u) scale_vec(0, u);
+      } else {
+#pragma unroll
+        for (int u = 0; u < SW; ++u) scale_word(0, u);
+      }
+    }
   }
 #pragma unroll
-  for (int u = 0; u < FIRST; ++u) issue_copy(1 < KT ? 1 : KT - 1, 1, u);
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(FIRST) : "memory");
-  read_a(0, I0, I0);
-  read_b(0, I0, bx);
+  for (int u = 0; u < FIRST; ++u) issue_copy(NS - 1 < KT ? NS - 1 : KT - 1, NS - 1, u);
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * CH + FIRST) : "memory");
+  read_a(0, 0, I0, I0);
+  read_b(0, 0, I0, bx);
 
+  int st = 0, last = NS - 1;   // this step's stage, and the one whose copies are under way
   for (int kt = 0; kt < full; ++kt) {
-    const int st = kt & 1, next = kt + 1 < KT ? kt + 1 : KT - 1, after = kt + 2 < KT ? kt + 2 : KT - 1;
-    read_a(kt, I1, I0);
-    phase(I0, I0, 1, next, st ^ 1);
+    const int next = st + 1 == NS ? 0 : st + 1;
+    const int ahead = kt + NS - 1 < KT ? kt + NS - 1 : KT - 1, after = kt + NS < KT ? kt + NS : KT - 1;
+    read_a(kt, st, I1, I0);
+    phase(I0, I0, 1, ahead, last);
     issue_scales(kt);
-    read_a(kt, I0, I1);
-    read_b(kt, I1, bx);
-    phase(I1, I0, 2, next, st ^ 1);
-    read_a(kt, I1, I1);
+    read_a(kt, st, I0, I1);
+    read_b(kt, st, I1, bx);
+    phase(I1, I0, 2, ahead, last);
+    read_a(kt, st, I1, I1);
     phase(I0, I1, -1, 0, 0);
-    // all reads of this stage are issued; once they and this wave's copies of the next step are done, meet: behind the
-    // barrier the next stage is whole and this one is free
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    read_a(kt + 1, I0, I0);   // (behind the last step: read and not used)
-    read_b(kt + 1, I0, bx_next);
+    // all reads of this stage are issued; once they and this wave's copies of the next step are done (those of the NS - 2
+    // steps behind it may be under way), meet: behind the barrier the next stage is whole and this one is free
+    if (NS > 2 && t.vec_scales) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    asm volatile("s_barrier" ::: "memory");
+    read_a(kt + 1, next, I0, I0);   // (behind the last step: read and not used)
+    read_b(kt + 1, next, I0, bx_next);
     phase(I1, I1, 0, after, st);
 #pragma unroll
     for (int b = 0; b < TJ; ++b) bx[b] = bx_next[b];
+    last = st;
+    st = next;
   }
   if (half) {   // four blocks, one for each lane group
-    const char* s = smem + (full & 1) * STAGE;
+    const char* s = smem + st * STAGE;
     const int ah = mx_lds_offset(arow, frag_q), bh = OPER + mx_lds_offset(brow, frag_q);
     const char *axh = scale_at(as_off - frag_q, full), *bxh = scale_at(bs_off - frag_q, full);   // (byte q, not 2q)
 #pragma unroll
