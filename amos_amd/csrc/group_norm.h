@@ -53,17 +53,19 @@ struct GnStat {
   float n, mean, m2;
 };
 
-__device__ __forceinline__ float gn_silu_factor(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
+// 1 / (1 + exp(-z)), from z times -log2(e)
+__device__ __forceinline__ float gn_sigmoid2(float scaled) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(scaled)); }
+constexpr float kGnLog2e = 1.44269504088896341f;
 __device__ __forceinline__ float gn_act(float z, int act) {
   if (act == AMOS_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
-  if (act == AMOS_ACT_SILU) return z * gn_silu_factor(z);
+  if (act == AMOS_ACT_SILU) return z * gn_sigmoid2(z * -kGnLog2e);
   return z;
 }
-// dy act'(z)
-__device__ __forceinline__ float gn_act_gradient(float dy, float z, int act) {
+// dy act'(z); `scaled` = -log2(e) z (silu)
+__device__ __forceinline__ float gn_act_gradient(float dy, float z, float scaled, int act) {
   if (act == AMOS_ACT_RELU) return z > 0.f ? dy : 0.f;
   if (act == AMOS_ACT_SILU) {
-    const float s = gn_silu_factor(z);
+    const float s = gn_sigmoid2(scaled);
     return dy * (s * (1.f + z * (1.f - s)));
   }
   return dy;

@@ -5,20 +5,29 @@
 
 namespace amos {
 
-// what a lane needs of its channels: h = (x - mean) rstd, z = h weight + bias
+// What a lane needs of its channels.  With t = x - mean (a difference, not folded into a constant: the mean may be large)
+//   z = t a + bias, a = rstd weight;  -log2(e) z = t a2 + b2;  sums of d and of d t (times rstd: d h) are kept, and
+//   dx = d a - t rstd^2 E[d weight h] - rstd E[d weight] = d a - t k2 - k1:
+// the launches are bound by their arithmetic as much as by memory, and each element takes two operations fewer.
 template <int VEC>
 struct GnChannels {
-  float mean[VEC], rstd[VEC], weight[VEC], bias[VEC];
+  float mean[VEC], rstd[VEC], a[VEC], bias[VEC], a2[VEC], b2[VEC];
   __device__ __forceinline__ GnChannels(const GnParams& p, int n, int c0) {
+    load_run_any<VEC>(p.weight, c0, p.affine_dtype, 1.f, a);
+    load_run_any<VEC>(p.bias, c0, p.affine_dtype, 0.f, bias);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const int c = c0 + i;
-      const int64_t g = (int64_t)n * p.G + fast_div(c, p.by_cpg);
+      const int64_t g = (int64_t)n * p.G + fast_div(c0 + i, p.by_cpg);
       mean[i] = p.mean[g];
       rstd[i] = p.rstd[g];
+      a[i] *= rstd[i];
+      a2[i] = a[i] * -kGnLog2e;
+      b2[i] = bias[i] * -kGnLog2e;
     }
-    load_run_any<VEC>(p.weight, c0, p.affine_dtype, 1.f, weight);
-    load_run_any<VEC>(p.bias, c0, p.affine_dtype, 0.f, bias);
+  }
+  // d = dy act'(z) of channel i; t: x - mean
+  __device__ __forceinline__ float d(int i, float t, float dy, int act) const {
+    return gn_act_gradient(dy, t * a[i] + bias[i], t * a2[i] + b2[i], act);
   }
 };
 
@@ -53,17 +62,17 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_partial(const GnP
         DenseVec<YT, VEC>::widen(rg[u], g);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          const float h = (v[i] - ch.mean[i]) * ch.rstd[i];
-          const float d = gn_act_gradient(g[i], h * ch.weight[i] + ch.bias[i], p.act);
+          const float t = v[i] - ch.mean[i];
+          const float d = ch.d(i, t, g[i], p.act);
           a1[i] += d;
-          a2[i] += d * h;
+          a2[i] += d * t;
         }
       }
     }
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       s1[(w.row * p.cols + w.col) * VEC + i] = a1[i];
-      s2[(w.row * p.cols + w.col) * VEC + i] = a2[i];
+      s2[(w.row * p.cols + w.col) * VEC + i] = a2[i] * ch.rstd[i];
     }
   }
   __syncthreads();
@@ -174,8 +183,8 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_apply(const GnPar
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     const int g = fast_div(w.c0 + w.col * VEC + i, p.by_cpg) - w.g0;
-    e1[i] = s1[g];
-    e2[i] = s2[g];
+    e1[i] = s1[g] * ch.rstd[i];
+    e2[i] = s2[g] * ch.rstd[i] * ch.rstd[i];
   }
   const int64_t base = w.n * p.image + w.c0 + w.col * VEC;
   const typename XT::raw_t* const x = (const typename XT::raw_t*)p.x + base;
@@ -199,9 +208,8 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_apply(const GnPar
       DenseVec<YT, VEC>::widen(rg[u], g);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float h = (v[i] - ch.mean[i]) * ch.rstd[i];
-        const float d = gn_act_gradient(g[i], h * ch.weight[i] + ch.bias[i], p.act);
-        v[i] = (d * ch.weight[i] - e1[i] - h * e2[i]) * ch.rstd[i];
+        const float t = v[i] - ch.mean[i];
+        v[i] = ch.d(i, t, g[i], p.act) * ch.a[i] - (t * e2[i] + e1[i]);
       }
       DenseVec<XT, VEC>::store(dx + (int64_t)(q + u * p.rows) * p.pixel, v);
     }
@@ -242,16 +250,16 @@ __global__ __launch_bounds__(1024) void amos_gn_gradient_held(const GnParams p) 
       VY::widen(rg[r], g);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        const float h = (v[i] - ch.mean[i]) * ch.rstd[i];
-        const float d = gn_act_gradient(g[i], h * ch.weight[i] + ch.bias[i], p.act);
+        const float t = v[i] - ch.mean[i];
+        const float d = ch.d(i, t, g[i], p.act);
         a1[i] += d;
-        a2[i] += d * h;
+        a2[i] += d * t;
       }
     }
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
       s1[w.row * p.ct + w.col * VEC + i] = a1[i];
-      s2[w.row * p.ct + w.col * VEC + i] = a2[i];
+      s2[w.row * p.ct + w.col * VEC + i] = a2[i] * ch.rstd[i];
     }
   }
   __syncthreads();
@@ -318,8 +326,8 @@ __global__ __launch_bounds__(1024) void amos_gn_gradient_held(const GnParams p) 
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
     const int g = fast_div(w.c + i, p.by_cpg) - w.g0;
-    m1[i] = e1[g];
-    m2[i] = e2[g];
+    m1[i] = e1[g] * ch.rstd[i];
+    m2[i] = e2[g] * ch.rstd[i] * ch.rstd[i];
   }
 #pragma unroll
   for (int r = 0; r < R; ++r) {
@@ -330,9 +338,8 @@ __global__ __launch_bounds__(1024) void amos_gn_gradient_held(const GnParams p) 
     VY::widen(rg[r], g);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) {
-      const float h = (v[i] - ch.mean[i]) * ch.rstd[i];
-      const float d = gn_act_gradient(g[i], h * ch.weight[i] + ch.bias[i], p.act);
-      v[i] = (d * ch.weight[i] - m1[i] - h * m2[i]) * ch.rstd[i];
+      const float t = v[i] - ch.mean[i];
+      v[i] = ch.d(i, t, g[i], p.act) * ch.a[i] - (t * m2[i] + m1[i]);
     }
     VX::store((typename XT::raw_t*)p.out + base + (int64_t)q * p.pixel, v);
   }
