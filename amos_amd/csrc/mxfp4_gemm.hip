@@ -229,12 +229,14 @@ static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   return 0;
 }
 
-// The tile by how many there are: 64x64 (four waves, four stages, two workgroups a compute unit) while one round takes
+// The tile: 32x64 for up to 32 rows of A (24 x 10240 x 8192: 13.1 us, 64x64 15.3, the few-rows kernel 15.5), else by how many
+// there are: 64x64 (four waves, four stages, two workgroups a compute unit) while one round takes
 // them or one side has no more rows (2048 x 1024 x 4096: 12.7 us, 128x128 16.4; 4096 x 1024 x 2048, 1024 of them: 15.0 / 11.7);
 // 128x128 in one round with four waves and three stages (4096 x 1024 x 2048: 11.7 us, eight waves 11.8; 1024 x 4096 x 4096:
 // 17.8 / 19.2), beyond that with eight waves and two workgroups a compute unit (4096 x 2048 x 1024: 12.1 us, four waves 13.4);
 // 256x256 from a full round on (4096 x 4096 x 1024: 17.1 us, 128x128 19.9).
 static int pick_tile(const MxGemmParams& p, hipStream_t stream) {
+  if (p.M <= 32) return launch_tile<1, 4, 32, 64, 4>(p, stream);
   const auto tiles = [&](int64_t e) { return (p.M + e - 1) / e * ((p.N + e - 1) / e); };
   if (tiles(64) <= 512 || p.M <= 64 || p.N <= 64) return launch_tile<2, 2, 64, 64, 4>(p, stream);
   if (tiles(128) <= 256) return launch_tile<2, 2, 128, 128, 3>(p, stream);
@@ -327,7 +329,7 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
     rc = pick_fused<SRC_F16>(p, blocks, stream);
   } else if (src == SRC_BF16) {
     rc = pick_fused<SRC_BF16>(p, blocks, stream);
-  } else if (d->M <= 16) {
+  } else if (d->M <= 16 && (blocks <= 768 || p.steps >= 1 << 18)) {   // (16384 rows of B: 9.0 us, 32x64 tiles 8.3)
     rc = pick_fused<SRC_MX>(p, blocks, stream);
   } else if (blocks <= 256 || p.steps >= 1 << 18) {
     rc = launch_few<SRC_MX, 1, 2>(p, stream);

@@ -48,8 +48,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   constexpr int SCALES = NS * STAGE, SPAN = (BI + BJ) * 32;      // behind them: two spans (four K steps) of scales
   constexpr int QA = BI / 8;
   constexpr int CH = (BI + BJ) / 8 / NW;                         // 1 KB copies of a wave and K step
-  constexpr int SV = (BI + BJ) / 32 / NW, SW = 4 * SV;           // copies of scales of a wave and span: 16 bytes a lane, 4 bytes
-  static_assert(CH >= 1 && CH * NW * 8 == BI + BJ && SV >= 1 && SV * NW * 32 == BI + BJ, "copies");
+  constexpr int SG = (BI + BJ) / 32, SV = (SG + NW - 1) / NW;     // copies of scales of a span, of a wave: 16 bytes a lane
+  constexpr int SW = CH;                                         // ... of a wave, 4 bytes a lane
+  static_assert(CH >= 1 && CH * NW * 8 == BI + BJ && BI % 32 == 0 && BJ % 32 == 0, "copies");
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const MxGemmParams& p = t.g;
   const int lane = threadIdx.x & 63;
@@ -98,6 +99,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   };
   auto scale_vec = [&](int span, int u) {      // 32 rows, two lanes a row
     const int first = (wave + NW * u) * 32, row = first + (lane >> 1);
+    if (SG % NW && first >= BI + BJ) return;
     const int want = span * 32 + ((lane ^ (row >> 3)) & 1) * 16;
     const unsigned char* base;
     const unsigned r = scale_row(row, base);
@@ -127,7 +129,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
         for (int u = 0; u < SV; ++u) scale_vec(span, u);
     } else {
 #pragma unroll
-      for (int u = 0; u < SW / 2; ++u) scale_word(span, (kt & 1) * (SW / 2) + u);
+      for (int u = 0; u < (SW + 1) / 2; ++u)
+        if ((kt & 1) * ((SW + 1) / 2) + u < SW) scale_word(span, (kt & 1) * ((SW + 1) / 2) + u);
     }
   };
 
@@ -225,8 +228,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     read_a(kt, st, I1, I1);
     phase(I0, I1, -1, 0, 0);
     // all reads of this stage are issued; once they and this wave's copies of the next step are done (those of the NS - 2
-    // steps behind it may be under way), meet: behind the barrier the next stage is whole and this one is free
-    if (NS > 2 && t.vec_scales) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
+    // steps behind it may be under way), meet: behind the barrier the next stage is whole and this one is free.  (Copies
+    // of one width complete in their order; for scales by words all are waited for once a span.)
+    if (NS > 2 && (t.vec_scales || (kt & 3) != 3)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     asm volatile("s_barrier" ::: "memory");
     read_a(kt + 1, next, I0, I0);   // (behind the last step: read and not used)
@@ -312,19 +316,20 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const int i0 = bi0 + (wi * TI + h * HA) * 16;
     if (out_dtype == AMOS_F32) {
-      constexpr int LPR = TJ * 4, RPI = 64 / LPR;
+      constexpr int LPR = TJ * 4, RPI = 64 / LPR < SR ? 64 / LPR : SR;   // lanes of a row, rows of an instruction
+      static_assert(SR % RPI == 0, "strip rows");
 #pragma unroll 2
       for (int n = 0; n < SR / RPI; ++n) {
         const int row = n * RPI + lane / LPR, col = (lane % LPR) * 4;
-        emit(i0 + row, wj0 + col, strip + row * SP + col, std::integral_constant<int, 4>{});
+        if (LPR * RPI == 64 || lane < LPR * RPI) emit(i0 + row, wj0 + col, strip + row * SP + col, std::integral_constant<int, 4>{});
       }
     } else {
-      constexpr int LPR = TJ * 2, RPI = 64 / LPR;
+      constexpr int LPR = TJ * 2, RPI = 64 / LPR < SR ? 64 / LPR : SR;
       static_assert(SR % RPI == 0, "strip rows");
 #pragma unroll 2
       for (int n = 0; n < SR / RPI; ++n) {
         const int row = n * RPI + lane / LPR, col = (lane % LPR) * 8;
-        emit(i0 + row, wj0 + col, strip + row * SP + col, std::integral_constant<int, 8>{});
+        if (LPR * RPI == 64 || lane < LPR * RPI) emit(i0 + row, wj0 + col, strip + row * SP + col, std::integral_constant<int, 8>{});
       }
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (the strip is read before it is written again)
