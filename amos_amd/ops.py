@@ -483,15 +483,6 @@ class Mxfp4(object):
             raise ValueError("codes are on %s, scales on %s" % (codes.device, scales.device))
         self.codes, self.scales, self.shape = codes, scales, (rows, int(cols))
 
-    @classmethod
-    def _empty(cls, rows, cols, like):
-        pitch = mxfp4_pitch(cols)
-        q = cls.__new__(cls)
-        q.codes = like.new_empty((rows, pitch), dtype=torch.uint8)
-        q.scales = like.new_empty((rows, pitch // 16), dtype=torch.uint8)
-        q.shape = (rows, cols)
-        return q
-
     @property
     def device(self):
         return self.codes.device
@@ -517,19 +508,17 @@ def _float_code(what, dtype):
     return code
 
 
-_current_device = torch.cuda.current_device
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # absent from a build without a GPU runtime
+# (of the module behind torch.cuda; absent from a build without a GPU runtime, where no tensor reaches them)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _on(body, device, stream, *args):
     """body(handle of the stream to launch on, *args) with `device` the current one and `stream` (None: the
     device's current one) current there, so that what the call allocates belongs to that stream's pool"""
-    index = device.index
     if stream is None:
-        if index == _current_device():
-            return body(_raw_stream(index), *args)
         with torch.cuda.device(device):
-            return body(_raw_stream(index), *args)
+            return body(_raw_stream(device.index), *args)
     if stream.device != device:
         raise ValueError("the stream belongs to %s, the tensors are on %s" % (stream.device, device))
     with torch.cuda.device(device), torch.cuda.stream(stream):
@@ -543,6 +532,8 @@ def _scratch(need, like):
 
 
 def _like_check(what, t, shape, device):
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.device == device and t.is_contiguous():
+        return
     _need_device(t)
     if t.shape != shape or t.device != device:
         raise ValueError("%s must be of shape %s on %s, got %s on %s" % (what, tuple(shape), device, tuple(t.shape), t.device))
@@ -558,7 +549,7 @@ class _Plans(dict):
         return plan
 
 
-_MX_GEMM_PLANS, _NORM_PLANS = _Plans(), _Plans()
+_MX_PLANS, _MX_GEMM_PLANS, _NORM_PLANS = _Plans(), _Plans(), _Plans()
 
 
 def mxfp4_quantize(x, axis=1, out=None, stream=None):
@@ -568,24 +559,34 @@ def mxfp4_quantize(x, axis=1, out=None, stream=None):
     [4, 8); elements are rounded to nearest even and saturate at 6; a block with an infinity or a NaN
     stands for NaN."""
     _need_device(x)
-    if x.dim() != 2 or x.numel() == 0:
-        raise ValueError("x must be a matrix with elements, got shape %s" % (tuple(x.shape),))
+    key = (x.shape, x.dtype, axis)
+    plan = _MX_PLANS.get(key) or _MX_PLANS.keep(key, _quantize_plan(*key))
+    if out is not None and (not isinstance(out, Mxfp4) or out.shape != plan[1] or out.device != x.device):
+        raise ValueError("out must be an Mxfp4 of shape %s on %s, got %r" % (plan[1], x.device, out))
+    index = x.get_device()
+    if stream is None and index == _current_device():
+        return _quantize(_raw_stream(index), plan, x, out)
+    return _on(_quantize, x.device, stream, plan, x, out)
+
+
+def _quantize_plan(shape, dtype, axis):
+    """(descriptor, shape of the result, of its codes, of its scales)"""
+    if len(shape) != 2 or 0 in shape:
+        raise ValueError("x must be a matrix with elements, got shape %s" % (tuple(shape),))
     if axis not in (0, 1, -1, -2):
         raise ValueError("axis %s of a matrix" % (axis,))
-    axis = axis % 2
-    rows, cols = x.shape
-    d = _lib.Mxfp4Desc(rows, cols, _float_code("x", x.dtype), axis)
-    if axis == 0:
-        rows, cols = cols, rows
-    if out is not None and (not isinstance(out, Mxfp4) or out.shape != (rows, cols) or out.device != x.device):
-        raise ValueError("out must be an Mxfp4 of shape %s on %s, got %r" % ((rows, cols), x.device, out))
-    return _on(_quantize, x.device, stream, x, d, rows, cols, out)
+    d = _lib.Mxfp4Desc(shape[0], shape[1], _float_code("x", dtype), axis % 2)
+    rows, cols = tuple(shape) if axis % 2 else (shape[1], shape[0])
+    pitch = mxfp4_pitch(cols)
+    return ctypes.byref(d), (rows, cols), (rows, pitch), (rows, pitch // 16)
 
 
-def _quantize(s, x, d, rows, cols, out):
+def _quantize(s, plan, x, out):
+    d, shape, codes, scales = plan
     if out is None:
-        out = Mxfp4._empty(rows, cols, x)
-    check(_lib.load().amos_mxfp4_quantize(ctypes.byref(d), x.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), s))
+        out = Mxfp4.__new__(Mxfp4)
+        out.codes, out.scales, out.shape = x.new_empty(codes, dtype=torch.uint8), x.new_empty(scales, dtype=torch.uint8), shape
+    check(_lib.load().amos_mxfp4_quantize(d, x.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), s))
     return out
 
 
@@ -597,6 +598,9 @@ def mxfp4_dequantize(q, dtype=torch.float32, out=None, stream=None):
         _need_device(out)
         _check_out(out, q.shape, dtype, q.codes)
     d = _lib.Mxfp4Desc(q.shape[0], q.shape[1], _float_code("the result", dtype), 1)
+    index = q.codes.get_device()
+    if stream is None and index == _current_device():
+        return _dequantize(_raw_stream(index), q, d, dtype, out)
     return _on(_dequantize, q.codes.device, stream, q, d, dtype, out)
 
 
@@ -635,6 +639,9 @@ def mxfp4_gemm(a, b, out=None, out_dtype=torch.float32, add=None, bias=None, str
             _like_check("the added operand", add, plan[1], device)
             epi.add, epi.add_dtype = add.data_ptr(), _float_code("the added operand", add.dtype)
         epi = ctypes.byref(epi)
+    index = device.index
+    if stream is None and index == _current_device():
+        return _mxfp4_gemm(_raw_stream(index), plan, a, b, dense, out, out_dtype, epi)
     return _on(_mxfp4_gemm, device, stream, plan, a, b, dense, out, out_dtype, epi)
 
 
@@ -645,7 +652,7 @@ def _mxfp4_gemm_plan(a_shape, b_shape, a_dtype, out_dtype):
     d = _lib.Mxfp4GemmDesc(a_shape[0], b_shape[0], b_shape[1], _lib.AMOS_MXFP4 if a_dtype is None else _float_code("a", a_dtype),
                            _float_code("the output", out_dtype))
     need = _lib.load().amos_mxfp4_gemm_workspace_bytes(ctypes.byref(d))
-    return d, (a_shape[0], b_shape[0]), need
+    return ctypes.byref(d), (a_shape[0], b_shape[0]), need
 
 
 def _mxfp4_gemm(s, plan, a, b, dense, out, out_dtype, epi):
@@ -654,7 +661,7 @@ def _mxfp4_gemm(s, plan, a, b, dense, out, out_dtype, epi):
         out = b.codes.new_empty(shape, dtype=out_dtype)
     ws, ws_ptr = _scratch(need, b.codes) if need else (None, None)
     ac, asc = (a.data_ptr(), None) if dense else (a.codes.data_ptr(), a.scales.data_ptr())
-    check(_lib.load().amos_mxfp4_gemm(ctypes.byref(d), epi, ac, asc, b.codes.data_ptr(), b.scales.data_ptr(), out.data_ptr(), ws_ptr, need, s))
+    check(_lib.load().amos_mxfp4_gemm(d, epi, ac, asc, b.codes.data_ptr(), b.scales.data_ptr(), out.data_ptr(), ws_ptr, need, s))
     return out
 
 
@@ -683,7 +690,7 @@ def _group_norm_plan(gradient, x_shape, x_dtype, y_dtype, groups, weight_dtype, 
         if t is not None:
             d.affine_dtype = _float_code("weight and bias", t)
     need = _lib.load().amos_group_norm_workspace_bytes(ctypes.byref(d), int(gradient))
-    return d, need, (ext["c"],), (ext["n"], groups)
+    return ctypes.byref(d), need, (ext["c"],), (ext["n"], groups)
 
 
 def _group_norm_key(gradient, x, y_dtype, groups, weight, bias, eps, activation, layout):
@@ -691,10 +698,11 @@ def _group_norm_key(gradient, x, y_dtype, groups, weight, bias, eps, activation,
     key = (gradient, x.shape, x.dtype, y_dtype, groups, None if weight is None else weight.dtype, None if bias is None else bias.dtype, eps,
            activation, layout)
     plan = _NORM_PLANS.get(key) or _NORM_PLANS.keep(key, _group_norm_plan(*key))
+    device = x.device
     if weight is not None:
-        _like_check("weight", weight, plan[2], x.device)
+        _like_check("weight", weight, plan[2], device)
     if bias is not None:
-        _like_check("bias", bias, plan[2], x.device)
+        _like_check("bias", bias, plan[2], device)
     return plan
 
 
@@ -718,6 +726,9 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, lay
     elif out_dtype is None:
         out_dtype = x.dtype
     plan = _group_norm_key(False, x, out_dtype, groups, weight, bias, eps, activation, layout)
+    index = x.get_device()
+    if stream is None and index == _current_device():
+        return _group_norm(_raw_stream(index), plan, x, weight, bias, out, out_dtype, stats)
     return _on(_group_norm, x.device, stream, plan, x, weight, bias, out, out_dtype, stats)
 
 
@@ -729,7 +740,7 @@ def _group_norm(s, plan, x, weight, bias, out, out_dtype, stats):
     if stats:
         mean, rstd = x.new_empty(stats_shape, dtype=torch.float32), x.new_empty(stats_shape, dtype=torch.float32)
     ws, ws_ptr = _scratch(need, x) if need else (None, None)
-    check(_lib.load().amos_group_norm(ctypes.byref(d), x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), _ptr(mean), _ptr(rstd), ws_ptr, need, s))
+    check(_lib.load().amos_group_norm(d, x.data_ptr(), _ptr(weight), _ptr(bias), out.data_ptr(), _ptr(mean), _ptr(rstd), ws_ptr, need, s))
     return (out, mean, rstd) if stats else out
 
 
@@ -743,6 +754,9 @@ def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, activ
     for what, t in (("mean", mean), ("rstd", rstd)):
         if t.shape != plan[3] or t.device != x.device or t.dtype != torch.float32:
             raise ValueError("%s must be fp32 of shape %s on %s, got %s %s on %s" % (what, plan[3], x.device, t.dtype, tuple(t.shape), t.device))
+    index = x.get_device()
+    if stream is None and index == _current_device():
+        return _group_norm_backward(_raw_stream(index), plan, dy, x, mean, rstd, weight, bias)
     return _on(_group_norm_backward, x.device, stream, plan, dy, x, mean, rstd, weight, bias)
 
 
@@ -752,7 +766,7 @@ def _group_norm_backward(s, plan, dy, x, mean, rstd, weight, bias):
     dweight = None if weight is None else x.new_empty(coefficients, dtype=torch.float32)
     dbias = None if bias is None else x.new_empty(coefficients, dtype=torch.float32)
     ws, ws_ptr = _scratch(need, x) if need else (None, None)
-    check(_lib.load().amos_group_norm_backward(ctypes.byref(d), dy.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias), mean.data_ptr(),
+    check(_lib.load().amos_group_norm_backward(d, dy.data_ptr(), x.data_ptr(), _ptr(weight), _ptr(bias), mean.data_ptr(),
                                                rstd.data_ptr(), dx.data_ptr(), _ptr(dweight), _ptr(dbias), ws_ptr, need, s))
     return dx, dweight, dbias
 
