@@ -42,6 +42,7 @@ struct GnParams {
   int slots;                 // partial results of a group: chunks * sub
   float eps;
   int act, affine_dtype;
+  float low;                 // act none, relu: what z is not let below
   FastDiv by_cpg, by_cols;
   FastDiv by_epg;            // one-launch kernels: entries of a group in a row of threads
   int y_dtype;
@@ -56,19 +57,21 @@ struct GnStat {
 // 1 / (1 + exp(-z)), from z times -log2(e)
 __device__ __forceinline__ float gn_sigmoid2(float scaled) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(scaled)); }
 constexpr float kGnLog2e = 1.44269504088896341f;
-__device__ __forceinline__ float gn_act(float z, int act) {
-  if (act == AMOS_ACT_RELU) return z > 0.f ? z : (z != z ? z : 0.f);
-  if (act == AMOS_ACT_SILU) return z * gn_sigmoid2(z * -kGnLog2e);
-  return z;
+// The activations without a branch an element: silu is a kernel's own instance; none and relu are z no lower than
+// `low`, -infinity or 0 (a comparison that is false for NaN: NaN stays)
+template <bool SILU>
+__device__ __forceinline__ float gn_act(float z, float low) {
+  if constexpr (SILU) return z * gn_sigmoid2(z * -kGnLog2e);
+  else return z < low ? low : z;
 }
-// dy act'(z); `scaled` = -log2(e) z (silu)
-__device__ __forceinline__ float gn_act_gradient(float dy, float z, float scaled, int act) {
-  if (act == AMOS_ACT_RELU) return z > 0.f ? dy : 0.f;
-  if (act == AMOS_ACT_SILU) {
-    const float s = gn_sigmoid2(scaled);
+template <bool SILU>
+__device__ __forceinline__ float gn_act_gradient(float dy, float z, float low) {   // dy act'(z)
+  if constexpr (SILU) {
+    const float s = gn_sigmoid2(z * -kGnLog2e);
     return dy * (s * (1.f + z * (1.f - s)));
+  } else {
+    return z > low ? dy : 0.f;
   }
-  return dy;
 }
 
 // where a workgroup works

@@ -1,0 +1,4 @@
+#include "group_norm_bwd_kernels.h"
+namespace amos {
+int group_norm_gradient_f16(const GnParams& p, const GnPlan& plan, hipStream_t stream) { return launch_gradient<TypeF16>(p, plan, stream); }
+}  // namespace amos

@@ -105,7 +105,7 @@ __device__ __forceinline__ void gn_join(const GnParams& p, int n, int g, int lan
 }
 
 // ---- second launch: normalise, scale, activate ----------------------------------------------------
-template <class XT, class YT, int VEC>
+template <class XT, class YT, int VEC, bool SILU>
 __global__ __launch_bounds__(kGnThreads) void amos_gn_apply(const GnParams p) {
   __shared__ float smean[kGnThreads * VEC], srstd[kGnThreads * VEC];   // by group of the tile
   const GnTile w = gn_tile<VEC>(p, blockIdx.x);
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_apply(const GnParams p) {
       float v[VEC];
       DenseVec<XT, VEC>::widen(raw[u], v);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] = gn_act((v[i] - m[i]) * a[i] + b[i], p.act);
+      for (int i = 0; i < VEC; ++i) v[i] = gn_act<SILU>((v[i] - m[i]) * a[i] + b[i], p.low);
       DenseVec<YT, VEC>::store(y + (int64_t)(q + u * p.rows) * p.pixel, v);
     }
   }
@@ -157,7 +157,7 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_apply(const GnParams p) {
     float v[VEC];
     DenseVec<XT, VEC>::load(x + (int64_t)q * p.pixel, v);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = gn_act((v[i] - m[i]) * a[i] + b[i], p.act);
+    for (int i = 0; i < VEC; ++i) v[i] = gn_act<SILU>((v[i] - m[i]) * a[i] + b[i], p.low);
     DenseVec<YT, VEC>::store(y + (int64_t)q * p.pixel, v);
   }
 }
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_apply(const GnParams p) {
 // ---- one launch: a slab of whole groups stays in registers between the sums and the output -----------
 // One pass over memory.  A thread holds R vectors of 16 bytes (all its loads are in flight together); mean, then the
 // squared deviations from it, from the registers.
-template <class XT, int VEC, int R, bool UNI>
+template <class XT, int VEC, int R, bool UNI, bool SILU>
 __global__ __launch_bounds__(1024) void amos_gn_held(const GnParams p) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   typedef DenseVec<XT, VEC> V;
@@ -246,31 +246,32 @@ __global__ __launch_bounds__(1024) void amos_gn_held(const GnParams p) {
     float v[VEC];
     V::widen(raw[r], v);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) v[i] = gn_act((v[i] - mean[UNI ? 0 : i]) * gamma[i] + beta[i], p.act);
+    for (int i = 0; i < VEC; ++i) v[i] = gn_act<SILU>((v[i] - mean[UNI ? 0 : i]) * gamma[i] + beta[i], p.low);
     store_run_any<VEC>(p.out, w.n * p.image + w.c + (int64_t)q * p.pixel, p.y_dtype, v);
   }
 }
 
-template <class XT, int VEC, bool UNI>
+template <class XT, int VEC, bool UNI, bool SILU>
 static void launch_held(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)p.N * p.tiles)), block((unsigned)plan.threads);
-  if (plan.held <= 4) hipLaunchKernelGGL((amos_gn_held<XT, VEC, 4, UNI>), grid, block, plan.lds, stream, p);
-  else hipLaunchKernelGGL((amos_gn_held<XT, VEC, kGnHeldForward, UNI>), grid, block, plan.lds, stream, p);
+  if (plan.held <= 4) hipLaunchKernelGGL((amos_gn_held<XT, VEC, 4, UNI, SILU>), grid, block, plan.lds, stream, p);
+  else hipLaunchKernelGGL((amos_gn_held<XT, VEC, kGnHeldForward, UNI, SILU>), grid, block, plan.lds, stream, p);
 }
-template <class XT>
+template <class XT, bool SILU>
 static void pick_held(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
   if constexpr (XT::ES == 2) {
-    if (plan.vec == 8) return plan.uni ? launch_held<XT, 8, true>(p, plan, stream) : launch_held<XT, 8, false>(p, plan, stream);
+    if (plan.vec == 8) return plan.uni ? launch_held<XT, 8, true, SILU>(p, plan, stream) : launch_held<XT, 8, false, SILU>(p, plan, stream);
   }
-  if (plan.vec == 4) return plan.uni ? launch_held<XT, 4, true>(p, plan, stream) : launch_held<XT, 4, false>(p, plan, stream);
-  launch_held<XT, 1, true>(p, plan, stream);
+  if (plan.vec == 4) return plan.uni ? launch_held<XT, 4, true, SILU>(p, plan, stream) : launch_held<XT, 4, false, SILU>(p, plan, stream);
+  launch_held<XT, 1, true, SILU>(p, plan, stream);
 }
 
 template <class XT, class YT, int VEC>
 static void launch(const GnParams& p, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)p.N * p.chunks), (unsigned)p.tiles), block(kGnThreads);
   hipLaunchKernelGGL((amos_gn_partial<XT, VEC>), grid, block, 0, stream, p);
-  hipLaunchKernelGGL((amos_gn_apply<XT, YT, VEC>), grid, block, 0, stream, p);
+  if (p.act == AMOS_ACT_SILU) hipLaunchKernelGGL((amos_gn_apply<XT, YT, VEC, true>), grid, block, 0, stream, p);
+  else hipLaunchKernelGGL((amos_gn_apply<XT, YT, VEC, false>), grid, block, 0, stream, p);
 }
 template <class XT, class YT>
 static void pick_vec(const GnParams& p, int vec, hipStream_t stream) {
@@ -298,9 +299,10 @@ static int run_forward(const amos_group_norm_desc_t* d, const void* x, const voi
   p.mean = mean;
   p.rstd = rstd;
   if (plan.held) {
-    if (d->x_dtype == AMOS_F32) pick_held<TypeF32>(p, plan, stream);
-    else if (d->x_dtype == AMOS_F16) pick_held<TypeF16>(p, plan, stream);
-    else pick_held<TypeBF16>(p, plan, stream);
+    const bool silu = p.act == AMOS_ACT_SILU;
+    if (d->x_dtype == AMOS_F32) silu ? pick_held<TypeF32, true>(p, plan, stream) : pick_held<TypeF32, false>(p, plan, stream);
+    else if (d->x_dtype == AMOS_F16) silu ? pick_held<TypeF16, true>(p, plan, stream) : pick_held<TypeF16, false>(p, plan, stream);
+    else silu ? pick_held<TypeBF16, true>(p, plan, stream) : pick_held<TypeBF16, false>(p, plan, stream);
   } else if (d->x_dtype == AMOS_F32) {
     pick_out<TypeF32>(p, plan.vec, d->y_dtype, stream);
   } else if (d->x_dtype == AMOS_F16) {

@@ -142,6 +142,7 @@ inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<const
   p.pixel = d->layout == AMOS_LAYOUT_NHWC ? p.C : (int64_t)p.N * p.C;
   p.eps = d->eps;
   p.act = d->activation;
+  p.low = d->activation == AMOS_ACT_RELU ? 0.f : -__builtin_inff();
   p.affine_dtype = d->affine_dtype;
   p.y_dtype = d->y_dtype;
   p.weight = weight;
