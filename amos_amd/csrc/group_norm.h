@@ -48,12 +48,6 @@ struct GnParams {
   int y_dtype;
 };
 
-// sums over the pixels of one group are kept as (count, mean, sum of squared deviations): no
-// difference of large sums, whatever the mean is
-struct GnStat {
-  float n, mean, m2;
-};
-
 // 1 / (1 + exp(-z)), from z times -log2(e)
 __device__ __forceinline__ float gn_sigmoid2(float scaled) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(scaled)); }
 constexpr float kGnLog2e = 1.44269504088896341f;

@@ -4,6 +4,7 @@
 namespace amos {
 
 // ---- first launch: a chunk's (count, mean, squared deviations) for every group of the tile --------
+// (no difference of large sums, whatever the mean is)
 template <class XT, int VEC>
 __global__ __launch_bounds__(kGnThreads) void amos_gn_partial(const GnParams p) {
   __shared__ float smean[kGnThreads * VEC], sm2[kGnThreads * VEC];

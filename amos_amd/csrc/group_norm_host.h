@@ -126,6 +126,8 @@ inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<const
   const int64_t lim = (int64_t)1 << 28;
   if (d->N >= lim || d->C >= lim || d->D >= lim || d->H >= lim || d->W >= lim || d->D * d->H >= lim || d->D * d->H * d->W >= lim)
     return set_error(AMOS_ERR_UNSUPPORTED, "group norm: images, channels or pixels of an image beyond 2^28");
+  if (d->N * (d->D * d->H * d->W) >= ((int64_t)1 << 40) / d->C)
+    return set_error(AMOS_ERR_UNSUPPORTED, "group norm: a tensor of 2^40 elements and more");
   if (d->layout != AMOS_LAYOUT_NHWC && d->layout != AMOS_LAYOUT_HWNC)
     return set_error(AMOS_ERR_UNSUPPORTED, "group norm: layout %d (channels-last layouts only)", d->layout);
   if (d->activation != AMOS_ACT_NONE && d->activation != AMOS_ACT_RELU && d->activation != AMOS_ACT_SILU)

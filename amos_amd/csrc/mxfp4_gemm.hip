@@ -220,12 +220,10 @@ static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   t.g = p;
   t.tiles_i = (p.M + BI - 1) / BI;
   t.tiles_j = (p.N + BJ - 1) / BJ;
-  t.per_split = (p.steps + 1) / 2;
-  t.slices = nullptr;
   t.stream_out = (int64_t)p.M * p.N * 4 > (int64_t)32 << 20;
   t.vec_scales = p.steps % 4 == 0 && (((uintptr_t)p.as | (uintptr_t)p.bs) & 15) == 0;
   if ((int64_t)t.tiles_i * t.tiles_j >= (int64_t)1 << 31) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d x %d results", p.M, p.N);
-  hipLaunchKernelGGL(fn, dim3((unsigned)(t.tiles_i * t.tiles_j), 1), dim3(64 * WI * WJ), lds, stream, t);
+  hipLaunchKernelGGL(fn, dim3((unsigned)(t.tiles_i * t.tiles_j)), dim3(64 * WI * WJ), lds, stream, t);
   return 0;
 }
 
@@ -250,8 +248,8 @@ static int check_desc(const amos_mxfp4_gemm_desc_t* d) {
   if (!d) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
   if (d->M < 1 || d->N < 1 || d->K < 1)
     return set_error(AMOS_ERR_BAD_ARG, "4-bit product of extents M %lld, N %lld, K %lld", (long long)d->M, (long long)d->N, (long long)d->K);
-  const int64_t lim = (int64_t)1 << 31;
-  if (d->M >= lim || d->N >= lim || d->K >= lim) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product: extents of 2^31 and more");
+  if (d->M >= (int64_t)1 << 30 || d->N >= (int64_t)1 << 30 || d->K >= (int64_t)1 << 31)
+    return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product: M or N of 2^30 and more, or K of 2^31 and more");
   if (d->a_dtype != AMOS_MXFP4 && !is_dense_dtype(d->a_dtype))
     return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product: A of dtype %d (4 bits, fp32, fp16 or bf16)", d->a_dtype);
   if (!is_dense_dtype(d->out_dtype)) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product: output dtype %d (fp32, fp16 or bf16)", d->out_dtype);
@@ -329,9 +327,9 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
     rc = pick_fused<SRC_F16>(p, blocks, stream);
   } else if (src == SRC_BF16) {
     rc = pick_fused<SRC_BF16>(p, blocks, stream);
-  } else if (d->M <= 16 && (blocks <= 768 || p.steps >= 1 << 18)) {   // (16384 rows of B: 9.0 us, 32x64 tiles 8.3)
+  } else if (d->M <= 16 && (blocks <= 768 || p.steps >= 1 << 16)) {   // (16384 rows of B: 9.0 us, 32x64 tiles 8.3)
     rc = pick_fused<SRC_MX>(p, blocks, stream);
-  } else if (blocks <= 256 || p.steps >= 1 << 18) {
+  } else if (blocks <= 256 || p.steps >= 1 << 16) {
     rc = launch_few<SRC_MX, 1, 2>(p, stream);
   } else if (blocks <= 512) {
     rc = launch_few<SRC_MX, 2, 2>(p, stream);

@@ -23,8 +23,6 @@ namespace amos {
 struct MxTileParams {
   MxGemmParams g;
   int tiles_i, tiles_j;
-  int per_split;        // K steps of a split (blockIdx.y); its sums go to `slices` + y * M * N, fp32
-  float* slices;        // null: not split
   int vec_scales;       // rows of scales are whole 16-byte pieces from 16-byte aligned memory on
   int stream_out;       // an fp32 C larger than the L2s together: written past them (8192^3: 281 -> 270 us)
 };
@@ -60,15 +58,12 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   block_to_tile(blockIdx.x, gridDim.x, t.tiles_i, t.tiles_j, tile_i, tile_j);
   const int bi0 = tile_i * BI, bj0 = tile_j * BJ;
   const int64_t pitch = (int64_t)p.steps * 64, spitch = (int64_t)p.steps * 4;
-  const int kt0 = (int)blockIdx.y * t.per_split;
-  const unsigned char* const abase = p.a + bi0 * pitch + (int64_t)kt0 * 128;
-  const unsigned char* const bbase = p.b + bj0 * pitch + (int64_t)kt0 * 128;
-  const unsigned char* const asbase = p.as + bi0 * spitch + (int64_t)kt0 * 8;
-  const unsigned char* const bsbase = p.bs + bj0 * spitch + (int64_t)kt0 * 8;
-  // this block's whole K steps, and whether a half one follows
-  int steps = p.steps - 2 * kt0;
-  if (steps > 2 * t.per_split) steps = 2 * t.per_split;
-  const int full = steps >> 1, half = steps & 1, KT = full + half;
+  const unsigned char* const abase = p.a + bi0 * pitch;
+  const unsigned char* const bbase = p.b + bj0 * pitch;
+  const unsigned char* const asbase = p.as + bi0 * spitch;
+  const unsigned char* const bsbase = p.bs + bj0 * spitch;
+  // whole K steps, and whether a half one follows
+  const int full = p.steps >> 1, half = p.steps & 1, KT = full + half;
 
   unsigned g_off[CH];
   const int chunk = (lane & 7) ^ (((lane >> 3) ^ (wave & 1)) & 7);   // (NW even: the same for every copy of the wave)
@@ -93,17 +88,15 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   // Scales: a row's 32 bytes of four K steps at once (8 bytes a row and step would touch as many memory lines per
   // step as the codes do).  Bit 3 of the row swaps the two 16-byte halves of its place: sixteen rows on different
   // banks.  What lies behind a row's end is fetched from its last bytes (and not used).
-  auto scale_row = [&](int row, const unsigned char*& base) -> unsigned {   // row of the tile (A's, then B's) -> row in memory
-    base = row < BI ? asbase : bsbase;
+  auto scale_row = [&](int row) -> unsigned {   // row of the tile (A's, then B's) -> row of its operand, from the tile's first on
     return (unsigned)(row < BI ? (bi0 + row < p.M ? row : p.M - 1 - bi0) : (bj0 + row - BI < p.N ? row - BI : p.N - 1 - bj0));
   };
   auto scale_vec = [&](int span, int u) {      // 32 rows, two lanes a row
     const int first = (wave + NW * u) * 32, row = first + (lane >> 1);
     if (SG % NW && first >= BI + BJ) return;
     const int want = span * 32 + ((lane ^ (row >> 3)) & 1) * 16;
-    const unsigned char* base;
-    const unsigned r = scale_row(row, base);
-    const int last = (int)spitch - kt0 * 8 - 16;
+    const unsigned r = scale_row(row);
+    const int last = (int)spitch - 16;
     const unsigned off = r * (unsigned)spitch + (unsigned)(want < last ? want : last);
     const unsigned char* const sb = first < BI ? asbase : bsbase;
     asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + SCALES + (span & 1) * SPAN + first * 32), "v"(off), "s"(sb) : "memory");
@@ -111,9 +104,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   auto scale_word = [&](int span, int u) {     // 8 rows, eight lanes a row
     const int first = (wave + NW * u) * 8, row = first + (lane >> 3);
     const int want = span * 8 + ((lane & 7) ^ (((row >> 3) & 1) << 2));
-    const unsigned char* base;
-    const unsigned r = scale_row(row, base);
-    const int last = p.steps - kt0 * 2 - 1;
+    const unsigned r = scale_row(row);
+    const int last = p.steps - 1;
     const unsigned off = r * (unsigned)spitch + (unsigned)(want < last ? want : last) * 4;
     const unsigned char* const sb = first < BI ? asbase : bsbase;
     asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds0 + SCALES + (span & 1) * SPAN + first * 32), "v"(off), "s"(sb) : "memory");
@@ -265,11 +257,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   constexpr int SP = TJ * 16 + 4, SR = HA * 16;
   static_assert(NW * SR * SP * 4 <= SCALES + 2 * SPAN, "output strip");
   float* const strip = (float*)smem + wave * (SR * SP);
-  const bool split = t.slices != nullptr;
-  void* const out = split ? (void*)(t.slices + (int64_t)blockIdx.y * p.M * p.N) : p.c;
-  const int out_dtype = split ? (int)AMOS_F32 : p.out_dtype;
   const int wj0 = bj0 + wj * TJ * 16;
-  const bool bias = !split && p.tail.bias, add = !split && p.tail.add;
   // V neighbouring results of a lane
   auto emit = [&](int i, int j, const float* from, auto width) {
     constexpr int V = decltype(width)::value;
@@ -283,27 +271,27 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     const int64_t at = (int64_t)i * p.N + j;
     if (i >= p.M || j >= p.N) return;
     if (j + V <= p.N) {
-      if (bias) {
+      if (p.tail.bias) {
         load_run_any<V>(p.tail.bias, j, p.tail.bias_dtype, 0.f, e);
 #pragma unroll
         for (int x = 0; x < V; ++x) v[x] += e[x];
       }
-      if (add) {
+      if (p.tail.add) {
         load_run_any<V>(p.tail.add, at, p.tail.add_dtype, 0.f, e);
 #pragma unroll
         for (int x = 0; x < V; ++x) v[x] += e[x];
       }
       if constexpr (V == 4) {
-        if (t.stream_out) DenseVec<TypeF32, 4>::store_streaming((float*)out + at, v);
-        else DenseVec<TypeF32, 4>::store((float*)out + at, v);
+        if (t.stream_out) DenseVec<TypeF32, 4>::store_streaming((float*)p.c + at, v);
+        else DenseVec<TypeF32, 4>::store((float*)p.c + at, v);
       } else {
-        if (out_dtype == AMOS_F16) DenseVec<TypeF16, 8>::store((_Float16*)out + at, v);
-        else DenseVec<TypeBF16, 8>::store((__bf16*)out + at, v);
+        if (p.out_dtype == AMOS_F16) DenseVec<TypeF16, 8>::store((_Float16*)p.c + at, v);
+        else DenseVec<TypeBF16, 8>::store((__bf16*)p.c + at, v);
       }
     } else {
 #pragma unroll
       for (int x = 0; x < V; ++x)
-        if (j + x < p.N) store_any(out, at + x, out_dtype, split ? v[x] : mx_tail(p.tail, v[x], i, j + x, p.N));
+        if (j + x < p.N) store_any(p.c, at + x, p.out_dtype, mx_tail(p.tail, v[x], i, j + x, p.N));
     }
   };
   auto store_half = [&](int h) {
@@ -315,7 +303,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
         for (int r = 0; r < 4; ++r) strip[(a * 16 + 4 * frag_q + r) * SP + b * 16 + frag_row] = acc[h * HA + a][b][r];
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     const int i0 = bi0 + (wi * TI + h * HA) * 16;
-    if (out_dtype == AMOS_F32) {
+    if (p.out_dtype == AMOS_F32) {
       constexpr int LPR = TJ * 4, RPI = 64 / LPR < SR ? 64 / LPR : SR;   // lanes of a row, rows of an instruction
       static_assert(SR % RPI == 0, "strip rows");
 #pragma unroll 2

@@ -59,6 +59,7 @@ def test_dequantize_refuses_the_other_axis():
 @pytest.mark.parametrize("change, code, text", [
     (dict(M=0), _lib.AMOS_ERR_BAD_ARG, "extents"),
     (dict(K=1 << 31), _lib.AMOS_ERR_UNSUPPORTED, "2^31"),
+    (dict(N=1 << 30), _lib.AMOS_ERR_UNSUPPORTED, "2^30"),
     (dict(a_dtype=_lib.AMOS_I8), _lib.AMOS_ERR_UNSUPPORTED, "A of dtype"),
     (dict(out_dtype=_lib.AMOS_I32), _lib.AMOS_ERR_UNSUPPORTED, "output dtype"),
     (dict(A=None), _lib.AMOS_ERR_BAD_ARG, "null"),
@@ -110,6 +111,7 @@ def norm_desc(**change):
     (dict(eps=-1.0), _lib.AMOS_ERR_BAD_ARG, "eps"),
     (dict(eps=float("nan")), _lib.AMOS_ERR_BAD_ARG, "eps"),
     (dict(H=1 << 20, W=1 << 20), _lib.AMOS_ERR_UNSUPPORTED, "2^28"),
+    (dict(N=1 << 20, H=1 << 12, C=1 << 12), _lib.AMOS_ERR_UNSUPPORTED, "2^40"),
 ])
 def test_group_norm_refuses(change, code, text):
     lib = _lib.load()
