@@ -1,9 +1,8 @@
 // Kernels of the group norm gradient; one translation unit for each type of x (group_norm_bwd_*.hip).
 #pragma once
-#include <mutex>
-
 #include "group_norm.h"
 #include "group_norm_host.h"
+#include "lds_limit.h"
 
 namespace amos {
 
@@ -363,10 +362,8 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_coefficients(const GnParam
 template <class XT, class YT, int VEC, int R, bool SILU>
 int launch_gradient_held(const GnParams& p, const GnPlan& plan, hipStream_t stream) {
   void (*const fn)(const GnParams) = amos_gn_gradient_held<XT, YT, VEC, R, SILU>;
-  static std::once_flag once;
-  static hipError_t err = hipSuccess;
-  std::call_once(once, [&] { err = hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024); });
-  if (err != hipSuccess) return set_error(AMOS_ERR_HIP, "hipFuncSetAttribute: %s", hipGetErrorString(err));
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_lds((const void*)fn, 96 * 1024, false, "amos_gn_gradient_held", done)) return rc;
   hipLaunchKernelGGL(fn, dim3((unsigned)((int64_t)p.N * p.tiles)), dim3((unsigned)plan.threads), plan.lds, stream, p);
   if (p.N > 1 && (p.dweight || p.dbias)) hipLaunchKernelGGL((amos_gn_coefficients<XT>), dim3((unsigned)((p.C + 15) / 16)), dim3(kGnThreads), 0, stream, p);
   return 0;

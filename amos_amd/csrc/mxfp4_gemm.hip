@@ -2,8 +2,7 @@
 
 #include <string.h>
 
-#include <mutex>
-
+#include "lds_limit.h"
 #include "mapper.h"
 #include "mxfp4_tile_kernel.h"
 
@@ -200,22 +199,12 @@ static int pick_fused(const MxGemmParams& p, int64_t blocks, hipStream_t stream)
 }
 
 // ---- many rows of A -----------------------------------------------------------------------------
-template <int WI, int WJ, int BI, int BJ, int NS>
+template <int WI, int WJ, int BI, int BJ, int NS, bool FLAT>
 static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   constexpr int lds = (BI + BJ) * (NS * 128 + 64);
-  void (*const fn)(const MxTileParams) = amos_mx_gemm_tile<WI, WJ, BI, BJ, NS>;
-  static std::once_flag once;
-  static hipError_t err = hipSuccess;
-  static int spilled = 0;
-  std::call_once(once, [&] {
-    err = hipFuncSetAttribute((const void*)fn, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    // (the kernel counts its outstanding copies; register spills would count among them)
-    hipFuncAttributes fa;
-    if (err == hipSuccess) err = hipFuncGetAttributes(&fa, (const void*)fn);
-    if (err == hipSuccess) spilled = (int)fa.localSizeBytes;
-  });
-  if (err != hipSuccess) return set_error(AMOS_ERR_HIP, "amos_mx_gemm_tile<%dx%d>: %s", BI, BJ, hipGetErrorString(err));
-  if (spilled) return set_error(AMOS_ERR_INFEASIBLE, "amos_mx_gemm_tile<%dx%d> was built with scratch memory", BI, BJ);
+  void (*const fn)(const MxTileParams) = amos_mx_gemm_tile<WI, WJ, BI, BJ, NS, FLAT>;
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_lds((const void*)fn, lds, true, "amos_mx_gemm_tile", done)) return rc;
   MxTileParams t;
   t.g = p;
   t.tiles_i = (p.M + BI - 1) / BI;
@@ -227,19 +216,19 @@ static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   return 0;
 }
 
-// The tile: 32x64 for up to 32 rows of A (24 x 10240 x 8192: 13.1 us, 64x64 15.3, the few-rows kernel 15.5), else by how many
+// The tile: 32x64 for up to 32 rows of A (24 x 10240 x 8192: 12.6 us, 64x64 15.1, the few-rows kernel 15.5), else by how many
 // there are: 64x64 (four waves, four stages, two workgroups a compute unit) while one round takes
-// them or one side has no more rows (2048 x 1024 x 4096: 12.7 us, 128x128 16.4; 4096 x 1024 x 2048, 1024 of them: 15.0 / 11.7);
+// them or one side has no more rows (2048 x 1024 x 4096: 13.4 us, 128x128 16.0; 4096 x 1024 x 2048, 1024 of them: 16.3 / 11.6);
 // 128x128 in one round with four waves and three stages (4096 x 1024 x 2048: 11.7 us, eight waves 11.8; 1024 x 4096 x 4096:
 // 17.8 / 19.2), beyond that with eight waves and two workgroups a compute unit (4096 x 2048 x 1024: 12.1 us, four waves 13.4);
 // 256x256 from a full round on (4096 x 4096 x 1024: 17.1 us, 128x128 19.9).
 static int pick_tile(const MxGemmParams& p, hipStream_t stream) {
-  if (p.M <= 32) return launch_tile<1, 4, 32, 64, 4>(p, stream);
+  if (p.M <= 32) return launch_tile<1, 4, 32, 64, 4, true>(p, stream);
   const auto tiles = [&](int64_t e) { return (p.M + e - 1) / e * ((p.N + e - 1) / e); };
-  if (tiles(64) <= 512 || p.M <= 64 || p.N <= 64) return launch_tile<2, 2, 64, 64, 4>(p, stream);
-  if (tiles(128) <= 256) return launch_tile<2, 2, 128, 128, 3>(p, stream);
-  if (tiles(256) < 256) return launch_tile<2, 4, 128, 128, 2>(p, stream);
-  return launch_tile<4, 2, 256, 256, 2>(p, stream);
+  if (tiles(64) <= 512 || p.M <= 64 || p.N <= 64) return launch_tile<2, 2, 64, 64, 4, true>(p, stream);
+  if (tiles(128) <= 256) return launch_tile<2, 2, 128, 128, 3, false>(p, stream);
+  if (tiles(256) < 256) return launch_tile<2, 4, 128, 128, 2, false>(p, stream);
+  return launch_tile<4, 2, 256, 256, 2, false>(p, stream);
 }
 
 int mx_quantize(const amos_mxfp4_desc_t* d, const void* x, void* codes, void* scales, hipStream_t stream);

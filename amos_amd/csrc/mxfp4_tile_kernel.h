@@ -36,7 +36,7 @@ __device__ __forceinline__ int mx_lds_offset(int row, int chunk) {
 
 #define AMOS_MX_LDS(p) ((__attribute__((address_space(3))) void*)(p))
 
-template <int WI, int WJ, int BI, int BJ, int NS>
+template <int WI, int WJ, int BI, int BJ, int NS, bool FLAT>
 __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTileParams t) {
   constexpr int NW = WI * WJ;
   constexpr int TI = BI / (16 * WI), TJ = BJ / (16 * WJ);
@@ -142,112 +142,178 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
 #pragma unroll
     for (int b = 0; b < TJ; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
 
-  mx_v4i af[2][HA], bf[2][TJ];      // A: by half of the wave tile's rows; B: by sub-step
-  int ax[TI], bx[TJ], bx_next[TJ];   // scales: a register serves both sub-steps
-  auto read_a = [&](int kt, int stage, auto h, auto ks) {
-    const char* s = smem + stage * STAGE;
-    const char* x = scale_at(as_off, kt);
-#pragma unroll
-    for (int a = 0; a < HA; ++a) {
-      af[h][a] = *(const mx_v4i*)(s + (a_off ^ (ks * 16)) + (h * HA + a) * 2048);
-      if (ks == 0) ax[h * HA + a] = *(const unsigned short*)(x + (h * HA + a) * 512);
-    }
-  };
-  auto read_b = [&](int kt, int stage, auto ks, int* to) {
-    const char* s = smem + stage * STAGE;
-    const char* x = scale_at(bs_off, kt);
-#pragma unroll
-    for (int b = 0; b < TJ; ++b) {
-      bf[ks][b] = *(const mx_v4i*)(s + (b_off ^ (ks * 16)) + b * 2048);
-      if (ks == 0) to[b] = *(const unsigned short*)(x + b * 512);
-    }
-  };
-  // One phase: the matrix instructions of half h of sub-step ks, and between them a share of the copies of step kt (a
-  // copy keeps its wave from issuing for some 64 cycles: spread out, the matrix core works through them).  The fences
-  // keep the compiler from moving the reads in front of a phase down to their use.
-  constexpr int SLOTS = 3 * TJ;   // places behind a group of HA instructions in the three phases that carry copies
-  auto phase = [&](auto h, auto ks, int part, int kt, int stage) {
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int b = 0; b < TJ; ++b) {
-#pragma unroll
-      for (int a = 0; a < HA; ++a) acc[h * HA + a][b] = mx_mfma<ks>(af[h][a], bf[ks][b], acc[h * HA + a][b], ax[h * HA + a], bx[b]);
-      if (part >= 0) {
-        const int slot = part * TJ + b;
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int u = slot * CH / SLOTS; u < (slot + 1) * CH / SLOTS; ++u) issue_copy(kt, stage, u);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);
-  };
   constexpr std::integral_constant<int, 0> I0{};
   constexpr std::integral_constant<int, 1> I1{};
-  constexpr int FIRST = TJ * CH / SLOTS;   // copies of part 0
-
-  // the first NS - 1 steps whole, of the next one the part that otherwise leaves in the step before
+  auto first_scales = [&]() {
+    if (t.vec_scales) {
 #pragma unroll
-  for (int s = 0; s < NS - 1; ++s) {
+      for (int u = 0; u < SV; ++u) scale_vec(0, u);
+    } else {
 #pragma unroll
-    for (int u = 0; u < CH; ++u) issue_copy(s < KT ? s : KT - 1, s, u);
-    if (s == 0) {
-      if (t.vec_scales) {
-#pragma unroll
-        for (int u = 0; u < SV; ++u) scale_vec(0, u);
-      } else {
-#pragma unroll
-        for (int u = 0; u < SW; ++u) scale_word(0, u);
-      }
+      for (int u = 0; u < SW; ++u) scale_word(0, u);
     }
-  }
+  };
+  int st = 0;   // this step's stage
+  if constexpr (FLAT) {
+    // Small wave tiles have too few matrix instructions a phase to hide an LDS read behind: all fragments of a step are
+    // read at once, a step ahead, into a second set of registers.
+    mx_v4i fa[2][2][TI], fb[2][2][TJ];
+    int xa[2][TI], xb[2][TJ];
+    auto read_all = [&](int kt, int stage, auto set) {
+      const char* s = smem + stage * STAGE;
+      const char *sa = scale_at(as_off, kt), *sb = scale_at(bs_off, kt);
 #pragma unroll
-  for (int u = 0; u < FIRST; ++u) issue_copy(NS - 1 < KT ? NS - 1 : KT - 1, NS - 1, u);
-  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * CH + FIRST) : "memory");
-  read_a(0, 0, I0, I0);
-  read_b(0, 0, I0, bx);
+      for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+        for (int a = 0; a < TI; ++a) fa[set][ks][a] = *(const mx_v4i*)(s + (a_off ^ (ks * 16)) + a * 2048);
+#pragma unroll
+        for (int b = 0; b < TJ; ++b) fb[set][ks][b] = *(const mx_v4i*)(s + (b_off ^ (ks * 16)) + b * 2048);
+      }
+#pragma unroll
+      for (int a = 0; a < TI; ++a) xa[set][a] = *(const unsigned short*)(sa + a * 512);
+#pragma unroll
+      for (int b = 0; b < TJ; ++b) xb[set][b] = *(const unsigned short*)(sb + b * 512);
+    };
+    auto step = [&](int kt, auto set, auto other) {
+      const int next = st + 1 == NS ? 0 : st + 1, after = kt + NS < KT ? kt + NS : KT - 1;
+      // this wave's copies of the next step have landed (those of the NS - 2 steps behind it may be under way; copies of
+      // one width complete in their order, for scales by words all are waited for once a span) and its reads of this
+      // one too: behind the barrier the next stage is whole and this one is free
+      if (NS > 2 && (t.vec_scales || (kt & 3) != 3)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      asm volatile("s_barrier" ::: "memory");
+      read_all(kt + 1, next, other);   // (behind the last step: read and not used)
+      __builtin_amdgcn_sched_barrier(0);
+      issue_scales(kt);
+#pragma unroll
+      for (int u = 0; u < CH; ++u) issue_copy(after, st, u);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int a = 0; a < TI; ++a)
+#pragma unroll
+        for (int b = 0; b < TJ; ++b) acc[a][b] = mx_mfma<0>(fa[set][0][a], fb[set][0][b], acc[a][b], xa[set][a], xb[set][b]);
+#pragma unroll
+      for (int a = 0; a < TI; ++a)
+#pragma unroll
+        for (int b = 0; b < TJ; ++b) acc[a][b] = mx_mfma<1>(fa[set][1][a], fb[set][1][b], acc[a][b], xa[set][a], xb[set][b]);
+      __builtin_amdgcn_sched_barrier(0);
+      st = next;
+    };
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+#pragma unroll
+      for (int u = 0; u < CH; ++u) issue_copy(s < KT ? s : KT - 1, s, u);
+      if (s == 0) first_scales();
+    }
+    if (t.vec_scales) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 1) * CH) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    read_all(0, 0, I0);
+    int kt = 0;
+    for (; kt + 1 < full; kt += 2) {
+      step(kt, I0, I1);
+      step(kt + 1, I1, I0);
+    }
+    if (kt < full) step(kt, I0, I1);
+  } else {
+    mx_v4i af[2][HA], bf[2][TJ];      // A: by half of the wave tile's rows; B: by sub-step
+    int ax[TI], bx[TJ], bx_next[TJ];   // scales: a register serves both sub-steps
+    auto read_a = [&](int kt, int stage, auto h, auto ks) {
+      const char* s = smem + stage * STAGE;
+      const char* x = scale_at(as_off, kt);
+#pragma unroll
+      for (int a = 0; a < HA; ++a) {
+        af[h][a] = *(const mx_v4i*)(s + (a_off ^ (ks * 16)) + (h * HA + a) * 2048);
+        if (ks == 0) ax[h * HA + a] = *(const unsigned short*)(x + (h * HA + a) * 512);
+      }
+    };
+    auto read_b = [&](int kt, int stage, auto ks, int* to) {
+      const char* s = smem + stage * STAGE;
+      const char* x = scale_at(bs_off, kt);
+#pragma unroll
+      for (int b = 0; b < TJ; ++b) {
+        bf[ks][b] = *(const mx_v4i*)(s + (b_off ^ (ks * 16)) + b * 2048);
+        if (ks == 0) to[b] = *(const unsigned short*)(x + b * 512);
+      }
+    };
+    // One phase: the matrix instructions of half h of sub-step ks, and between them a share of the copies of step kt (a
+    // copy keeps its wave from issuing for some 64 cycles: spread out, the matrix core works through them).  The fences
+    // keep the compiler from moving the reads in front of a phase down to their use.
+    constexpr int SLOTS = 3 * TJ;   // places behind a group of HA instructions in the three phases that carry copies
+    auto phase = [&](auto h, auto ks, int part, int kt, int stage) {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int b = 0; b < TJ; ++b) {
+#pragma unroll
+        for (int a = 0; a < HA; ++a) acc[h * HA + a][b] = mx_mfma<ks>(af[h][a], bf[ks][b], acc[h * HA + a][b], ax[h * HA + a], bx[b]);
+        if (part >= 0) {
+          const int slot = part * TJ + b;
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int u = slot * CH / SLOTS; u < (slot + 1) * CH / SLOTS; ++u) issue_copy(kt, stage, u);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    constexpr int FIRST = TJ * CH / SLOTS;   // copies of part 0
 
-  int st = 0, last = NS - 1;   // this step's stage, and the one whose copies are under way
-  for (int kt = 0; kt < full; ++kt) {
-    const int next = st + 1 == NS ? 0 : st + 1;
-    const int ahead = kt + NS - 1 < KT ? kt + NS - 1 : KT - 1, after = kt + NS < KT ? kt + NS : KT - 1;
-    read_a(kt, st, I1, I0);
-    phase(I0, I0, 1, ahead, last);
-    issue_scales(kt);
-    read_a(kt, st, I0, I1);
-    read_b(kt, st, I1, bx);
-    phase(I1, I0, 2, ahead, last);
-    read_a(kt, st, I1, I1);
-    phase(I0, I1, -1, 0, 0);
-    // all reads of this stage are issued; once they and this wave's copies of the next step are done (those of the NS - 2
-    // steps behind it may be under way), meet: behind the barrier the next stage is whole and this one is free.  (Copies
-    // of one width complete in their order; for scales by words all are waited for once a span.)
-    if (NS > 2 && (t.vec_scales || (kt & 3) != 3)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    asm volatile("s_barrier" ::: "memory");
-    read_a(kt + 1, next, I0, I0);   // (behind the last step: read and not used)
-    read_b(kt + 1, next, I0, bx_next);
-    phase(I1, I1, 0, after, st);
+    // the first NS - 1 steps whole, of the next one the part that otherwise leaves in the step before
 #pragma unroll
-    for (int b = 0; b < TJ; ++b) bx[b] = bx_next[b];
-    last = st;
-    st = next;
+    for (int s = 0; s < NS - 1; ++s) {
+#pragma unroll
+      for (int u = 0; u < CH; ++u) issue_copy(s < KT ? s : KT - 1, s, u);
+      if (s == 0) first_scales();
+    }
+#pragma unroll
+    for (int u = 0; u < FIRST; ++u) issue_copy(NS - 1 < KT ? NS - 1 : KT - 1, NS - 1, u);
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * CH + FIRST) : "memory");
+    read_a(0, 0, I0, I0);
+    read_b(0, 0, I0, bx);
+
+    int last = NS - 1;   // the stage whose copies are under way
+    for (int kt = 0; kt < full; ++kt) {
+      const int next = st + 1 == NS ? 0 : st + 1;
+      const int ahead = kt + NS - 1 < KT ? kt + NS - 1 : KT - 1, after = kt + NS < KT ? kt + NS : KT - 1;
+      read_a(kt, st, I1, I0);
+      phase(I0, I0, 1, ahead, last);
+      issue_scales(kt);
+      read_a(kt, st, I0, I1);
+      read_b(kt, st, I1, bx);
+      phase(I1, I0, 2, ahead, last);
+      read_a(kt, st, I1, I1);
+      phase(I0, I1, -1, 0, 0);
+      // all reads of this stage are issued; once they and this wave's copies of the next step are done (those of the NS - 2
+      // steps behind it may be under way), meet: behind the barrier the next stage is whole and this one is free.  (Copies
+      // of one width complete in their order; for scales by words all are waited for once a span.)
+      if (NS > 2 && (t.vec_scales || (kt & 3) != 3)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      asm volatile("s_barrier" ::: "memory");
+      read_a(kt + 1, next, I0, I0);   // (behind the last step: read and not used)
+      read_b(kt + 1, next, I0, bx_next);
+      phase(I1, I1, 0, after, st);
+#pragma unroll
+      for (int b = 0; b < TJ; ++b) bx[b] = bx_next[b];
+      last = st;
+      st = next;
+    }
   }
   if (half) {   // four blocks, one for each lane group
     const char* s = smem + st * STAGE;
     const int ah = mx_lds_offset(arow, frag_q), bh = OPER + mx_lds_offset(brow, frag_q);
     const char *axh = scale_at(as_off - frag_q, full), *bxh = scale_at(bs_off - frag_q, full);   // (byte q, not 2q)
+    mx_v4i g[TJ];
+    int y[TJ];
 #pragma unroll
     for (int b = 0; b < TJ; ++b) {
-      bf[0][b] = *(const mx_v4i*)(s + bh + b * 2048);
-      bx[b] = *(const unsigned char*)(bxh + b * 512);
+      g[b] = *(const mx_v4i*)(s + bh + b * 2048);
+      y[b] = *(const unsigned char*)(bxh + b * 512);
     }
 #pragma unroll
     for (int a = 0; a < TI; ++a) {
       const mx_v4i f = *(const mx_v4i*)(s + ah + a * 2048);
       const int x = *(const unsigned char*)(axh + a * 512);
 #pragma unroll
-      for (int b = 0; b < TJ; ++b) acc[a][b] = mx_mfma(f, bf[0][b], acc[a][b], x, bx[b]);
+      for (int b = 0; b < TJ; ++b) acc[a][b] = mx_mfma(f, g[b], acc[a][b], x, y[b]);
     }
   }
 
