@@ -42,7 +42,7 @@ struct GnParams {
   int slots;                 // partial results of a group: chunks * sub
   float eps;
   int act, affine_dtype;
-  float low;                 // act none, relu: what z is not let below
+  float low;                 // act none: NaN, relu: 0 (what z is not let below)
   FastDiv by_cpg, by_cols;
   FastDiv by_epg;            // one-launch kernels: entries of a group in a row of threads
   int y_dtype;
@@ -52,7 +52,7 @@ struct GnParams {
 __device__ __forceinline__ float gn_sigmoid2(float scaled) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(scaled)); }
 constexpr float kGnLog2e = 1.44269504088896341f;
 // The activations without a branch an element: silu is a kernel's own instance; none and relu are z no lower than
-// `low`, -infinity or 0 (a comparison that is false for NaN: NaN stays)
+// `low`, NaN or 0 (comparisons that are false for NaN: a z of NaN stays, and without an activation every z passes)
 template <bool SILU>
 __device__ __forceinline__ float gn_act(float z, float low) {
   if constexpr (SILU) return z * gn_sigmoid2(z * -kGnLog2e);
@@ -64,7 +64,7 @@ __device__ __forceinline__ float gn_act_gradient(float dy, float z, float low) {
     const float s = gn_sigmoid2(z * -kGnLog2e);
     return dy * (s * (1.f + z * (1.f - s)));
   } else {
-    return z > low ? dy : 0.f;
+    return z <= low ? 0.f : dy;
   }
 }
 

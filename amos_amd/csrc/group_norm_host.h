@@ -11,6 +11,7 @@ namespace amos {
 
 constexpr int kGnHeldForward = 16, kGnHeldGradient = 6;   // vectors a thread of the one-launch kernels holds at most
 constexpr int kGnHeldThreads = 1024;
+constexpr int64_t kGnGridThreads = (int64_t)1 << 32;   // a grid's first extent has fewer
 
 // The one-launch plan: as many groups a slab as bring a pixel's piece to 64 bytes (half a memory line), where
 // a workgroup's registers hold that much.
@@ -31,7 +32,6 @@ inline bool gn_plan_held(const amos_group_norm_desc_t* d, bool gradient, int vec
     if (p.C % (k * unit) == 0 && fits(k * unit)) ct = k * unit;
   // (measured on 32 x 56 x 56 x 256 bf16: pieces of 16 bytes 82 us where two launches over whole rows take half)
   if (ct * es < 64 && ct < p.C && (int64_t)p.N * p.P * p.C * es > (int64_t)4 << 20) return false;
-  if (p.N * (p.C / ct) >= (int64_t)1 << 31) return false;
   p.ct = (int)ct;
   p.tiles = (int)(p.C / ct);
   p.sub = p.chunks = 1;
@@ -53,7 +53,7 @@ inline bool gn_plan_held(const amos_group_norm_desc_t* d, bool gradient, int vec
   plan.lds = (p.rows * per * (gradient ? 2 : 1) + 2 * (p.ct / p.cpg)) * (int)sizeof(float);
   plan.part_floats = 0;
   plan.cpart_floats = gradient && p.N > 1 ? (int64_t)p.N * p.C * 2 : 0;   // the images' shares of dweight and dbias
-  return plan.lds <= 96 * 1024;
+  return plan.lds <= 96 * 1024 && p.N * (p.C / ct) * plan.threads < kGnGridThreads && (d->C / 16 + 1) * 256 < kGnGridThreads;
 }
 
 // The two-launch plan; 1: this vector length does not divide the tiles
@@ -96,7 +96,7 @@ inline int gn_plan_tiles(const amos_group_norm_desc_t* d, bool gradient, int vec
   if (chunk > P) chunk = P;
   p.chunk = (int)chunk;
   p.chunks = (int)((P + chunk - 1) / chunk);
-  if ((int64_t)p.N * p.chunks + C >= (int64_t)1 << 31) return set_error(AMOS_ERR_UNSUPPORTED, "group norm of %d images", p.N);
+  if (((int64_t)p.N * p.chunks + C / 16 + 1) * kGnThreads >= kGnGridThreads) return set_error(AMOS_ERR_UNSUPPORTED, "group norm of %d images", p.N);
   p.slots = p.chunks * p.sub;
   p.by_cols = make_fast_div((uint32_t)p.cols);
   p.by_cpg = make_fast_div((uint32_t)p.cpg);
@@ -144,7 +144,7 @@ inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<const
   p.pixel = d->layout == AMOS_LAYOUT_NHWC ? p.C : (int64_t)p.N * p.C;
   p.eps = d->eps;
   p.act = d->activation;
-  p.low = d->activation == AMOS_ACT_RELU ? 0.f : -__builtin_inff();
+  p.low = d->activation == AMOS_ACT_RELU ? 0.f : __builtin_nanf("");
   p.affine_dtype = d->affine_dtype;
   p.y_dtype = d->y_dtype;
   p.weight = weight;

@@ -189,6 +189,24 @@ def test_infinities_and_nan_stay_in_their_group(gpu):
     assert torch.equal(y.cpu()[~bad], clean.cpu()[~bad])
 
 
+@pytest.mark.parametrize("shape", [(2, 6, 7, 32), (2, 64, 64, 256)])       # one launch, two launches
+def test_gradient_without_an_activation_ignores_the_bias(gpu, shape):
+    """y's gradient by x does not know the bias, whatever it holds; relu stops at -infinity and passes NaN on"""
+    from amos_amd import ops
+    x, dy = make("nhwc", shape, 3).cuda(), make("nhwc", shape, 4).cuda()
+    w, b = (t.cuda() for t in coefficients(shape[-1], 3))
+    odd = b.clone()
+    odd[3], odd[17], odd[25] = float("nan"), float("-inf"), float("inf")
+    _, mean, rstd = ops.group_norm(x, 4, w, b, stats=True)
+    for one, two in zip(ops.group_norm_backward(dy, x, mean, rstd, 4, w, b), ops.group_norm_backward(dy, x, mean, rstd, 4, w, odd)):
+        assert torch.equal(one, two)
+    _, dw, db = ops.group_norm_backward(dy, x, mean, rstd, 4, w, odd, activation="relu")
+    plain, plain_b = ops.group_norm_backward(dy, x, mean, rstd, 4, w, b)[1:]
+    assert db[17] == 0 and dw[17] == 0
+    for c in (3, 25):
+        assert db[c] == plain_b[c] and dw[c] == plain[c]
+
+
 @pytest.mark.parametrize("shape, groups", [((2, 12, 11, 64), 8), ((1, 40, 50, 24), 3), ((4, 64, 64, 128), 32)])
 def test_in_place_misaligned_stream_and_repetition(gpu, shape, groups):
     from amos_amd import ops
