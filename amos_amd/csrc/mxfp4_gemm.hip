@@ -169,15 +169,17 @@ __global__ __launch_bounds__(64 * MAXW) void amos_mx_gemm_few(const MxGemmParams
   }
 }
 
+constexpr int64_t kGridThreads = (int64_t)1 << 32;   // a grid's first extent has fewer
 template <int SRC, int RT, int TT>
 static int launch_few(const MxGemmParams& p, hipStream_t stream) {
   constexpr int MAXW = TT == 1 ? 16 : 8;   // (the waves' sums: at most 64 KB)
   int waves = (p.steps + kTurn - 1) / kTurn;
   if (waves > MAXW) waves = MAXW;
   const int64_t gy = ((int64_t)p.M + 16 * TT - 1) / (16 * TT);
-  if (gy > 65535) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d rows and K %d", p.M, p.K);
+  const int64_t gx = ((int64_t)p.N + 16 * RT - 1) / (16 * RT);
+  if (gy > 65535 || gx * 64 * waves >= kGridThreads) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d x %d results and K %d", p.M, p.N, p.K);
   const size_t lds = waves > 1 ? (size_t)waves * RT * TT * 1024 : 0;
-  hipLaunchKernelGGL((amos_mx_gemm_few<SRC, RT, TT, MAXW>), dim3((unsigned)((p.N + 16 * RT - 1) / (16 * RT)), (unsigned)gy),
+  hipLaunchKernelGGL((amos_mx_gemm_few<SRC, RT, TT, MAXW>), dim3((unsigned)gx, (unsigned)gy),
                      dim3((unsigned)(64 * waves)), lds, stream, p);
   return 0;
 }
@@ -203,15 +205,15 @@ template <int WI, int WJ, int BI, int BJ, int NS, bool FLAT>
 static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   constexpr int lds = (BI + BJ) * (NS * 128 + 64);
   void (*const fn)(const MxTileParams) = amos_mx_gemm_tile<WI, WJ, BI, BJ, NS, FLAT>;
-  static std::atomic<uint64_t> done{0};
-  if (const int rc = allow_lds((const void*)fn, lds, true, "amos_mx_gemm_tile", done)) return rc;
   MxTileParams t;
   t.g = p;
   t.tiles_i = (p.M + BI - 1) / BI;
   t.tiles_j = (p.N + BJ - 1) / BJ;
   t.stream_out = (int64_t)p.M * p.N * 4 > (int64_t)32 << 20;
   t.vec_scales = p.steps % 4 == 0 && (((uintptr_t)p.as | (uintptr_t)p.bs) & 15) == 0;
-  if ((int64_t)t.tiles_i * t.tiles_j >= (int64_t)1 << 31) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d x %d results", p.M, p.N);
+  if ((int64_t)t.tiles_i * t.tiles_j * 64 * WI * WJ >= kGridThreads) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d x %d results", p.M, p.N);
+  static std::atomic<uint64_t> done{0};
+  if (const int rc = allow_lds((const void*)fn, lds, true, "amos_mx_gemm_tile", done)) return rc;
   hipLaunchKernelGGL(fn, dim3((unsigned)(t.tiles_i * t.tiles_j)), dim3(64 * WI * WJ), lds, stream, t);
   return 0;
 }

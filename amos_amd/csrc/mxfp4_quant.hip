@@ -187,20 +187,23 @@ int mx_quantize(const amos_mxfp4_desc_t* d, const void* x, void* codes, void* sc
   if (d->axis != 0) return set_error(AMOS_ERR_BAD_ARG, "quantisation along axis %d of a matrix", d->axis);
   QuantParams p;
   memset(&p, 0, sizeof(p));
-  p.codes = (unsigned char*)codes;
-  p.scales = (unsigned char*)scales;
-  p.rows = d->cols;
   p.cols = d->rows;
   p.ld = d->cols;
   p.pitch = mx_pitch(d->rows);
   const int64_t slabs = (d->rows + 255) / 256;   // of 256 rows of x: the grid's second extent
   if (slabs > 65535) return set_error(AMOS_ERR_UNSUPPORTED, "quantisation along axis 0 of more than %lld rows", 65535LL * 256);
-  p.x = x;
-  if (d->dtype == AMOS_F32) launch_columns<TypeF32>(p, (unsigned)slabs, stream);
-  else if (d->dtype == AMOS_F16) launch_columns<TypeF16>(p, (unsigned)slabs, stream);
-  else launch_columns<TypeBF16>(p, (unsigned)slabs, stream);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return set_error(AMOS_ERR_HIP, "launch failed: %s", hipGetErrorString(e));
+  constexpr int64_t most = (int64_t)1 << 24;     // columns of a launch: a grid has fewer than 2^32 threads
+  for (int64_t c = 0; c < d->cols; c += most) {
+    p.rows = d->cols - c < most ? d->cols - c : most;
+    p.x = (const char*)x + c * dense_size(d->dtype);
+    p.codes = (unsigned char*)codes + c * p.pitch;
+    p.scales = (unsigned char*)scales + c * (p.pitch / 16);
+    if (d->dtype == AMOS_F32) launch_columns<TypeF32>(p, (unsigned)slabs, stream);
+    else if (d->dtype == AMOS_F16) launch_columns<TypeF16>(p, (unsigned)slabs, stream);
+    else launch_columns<TypeBF16>(p, (unsigned)slabs, stream);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return set_error(AMOS_ERR_HIP, "launch failed: %s", hipGetErrorString(e));
+  }
   return 0;
 }
 

@@ -267,6 +267,22 @@ def test_more_than_32_bits_of_elements(gpu):
     assert big.shape == (1 << 20, 64) and not big.codes.any() and not big.scales.any()
 
 
+def test_columns_in_several_launches(gpu):
+    """axis 0 of a matrix wider than one launch takes"""
+    from amos_amd import ops
+    cols = (1 << 24) + 130
+    at = [0, 1, 63, (1 << 24) - 1, 1 << 24, (1 << 24) + 1, cols - 1]
+    x = torch.zeros(3, cols, dtype=torch.float16, device="cuda")
+    part = awkward(3, len(at), torch.float16)
+    x[:, at] = part.cuda()
+    q = ops.mxfp4_quantize(x, axis=0)
+    codes, scales = ref.quantize(part.t())
+    assert torch.equal(q.codes[at].cpu(), codes) and torch.equal(q.scales[at].cpu(), scales)
+    q.codes[at] = 0
+    q.scales[at] = 0
+    assert not q.codes.any() and not q.scales.any()
+
+
 def test_refusals_on_device_tensors(gpu):
     from amos_amd import ops
     x = torch.zeros(4, 64, device="cuda")

@@ -68,6 +68,8 @@ def test_dequantize_refuses_the_other_axis():
     (dict(B=AT + 4), _lib.AMOS_ERR_BAD_ARG, "16-byte"),
     (dict(b_scales=AT + 1), _lib.AMOS_ERR_BAD_ARG, "4-byte"),
     (dict(C=AT + 2), _lib.AMOS_ERR_BAD_ARG, "misaligned"),
+    (dict(N=(1 << 30) - 1), _lib.AMOS_ERR_UNSUPPORTED, "results"),          # grids of 2^32 threads and more
+    (dict(N=1 << 28, K=8192, a_dtype=_lib.AMOS_F32), _lib.AMOS_ERR_UNSUPPORTED, "results"),
     (dict(bias_dtype=_lib.AMOS_I8), _lib.AMOS_ERR_UNSUPPORTED, "bias"),
     (dict(add_dtype=_lib.AMOS_I32), _lib.AMOS_ERR_UNSUPPORTED, "added operand"),
 ])
@@ -112,6 +114,7 @@ def norm_desc(**change):
     (dict(eps=float("nan")), _lib.AMOS_ERR_BAD_ARG, "eps"),
     (dict(H=1 << 20, W=1 << 20), _lib.AMOS_ERR_UNSUPPORTED, "2^28"),
     (dict(N=1 << 20, H=1 << 12, C=1 << 12), _lib.AMOS_ERR_UNSUPPORTED, "2^40"),
+    (dict(N=1 << 26, H=1, W=1), _lib.AMOS_ERR_UNSUPPORTED, "images"),       # a grid of 2^32 threads
 ])
 def test_group_norm_refuses(change, code, text):
     lib = _lib.load()
