@@ -210,7 +210,7 @@ static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   t.tiles_i = (p.M + BI - 1) / BI;
   t.tiles_j = (p.N + BJ - 1) / BJ;
   t.stream_out = (int64_t)p.M * p.N * 4 > (int64_t)32 << 20;
-  t.vec_scales = p.steps % 4 == 0 && (((uintptr_t)p.as | (uintptr_t)p.bs) & 15) == 0;
+  t.vec_scales = p.steps >= 4;
   if ((int64_t)t.tiles_i * t.tiles_j * 64 * WI * WJ >= kGridThreads) return set_error(AMOS_ERR_UNSUPPORTED, "4-bit product of %d x %d results", p.M, p.N);
   static std::atomic<uint64_t> done{0};
   if (const int rc = allow_lds((const void*)fn, lds, true, "amos_mx_gemm_tile", done)) return rc;
@@ -218,18 +218,20 @@ static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   return 0;
 }
 
-// The tile: 32x64 for up to 32 rows of A (24 x 10240 x 8192: 12.6 us, 64x64 15.1, the few-rows kernel 15.5), else by how many
-// there are: 64x64 (four waves, four stages, two workgroups a compute unit) while one round takes
-// them or one side has no more rows (2048 x 1024 x 4096: 13.4 us, 128x128 16.0; 4096 x 1024 x 2048, 1024 of them: 16.3 / 11.6);
-// 128x128 in one round with four waves and three stages (4096 x 1024 x 2048: 11.7 us, eight waves 11.8; 1024 x 4096 x 4096:
-// 17.8 / 19.2), beyond that with eight waves and two workgroups a compute unit (4096 x 2048 x 1024: 12.1 us, four waves 13.4);
-// 256x256 from a full round on (4096 x 4096 x 1024: 17.1 us, 128x128 19.9).
+// The tile, by how many there are: 32x64 up to 32 rows of A (24 x 10240 x 8192: 12.6 us, 64x64 15.1, the few-rows kernel
+// 15.5) and while one round of the compute units takes them (333 x 1000 x 2050: 5.4 us, 64x64 6.2; 64 x 8192 x 4096, 256 tiles:
+// 7.5 / 8.7; 1000 x 1000 x 2048, 512: 6.4 / 6.2); 64x64 (two workgroups a compute unit) while one round takes
+// them or one side has no more rows (2048 x 1024 x 4096: 12.4 us, 128x128 17.3; 4096 x 1024 x 2048, 1024 of them: 15.6 / 11.5);
+// 128x128 in one round with four waves and three stages (4096 x 1024 x 2048: 11.5 us, eight waves 11.6; 1024 x 4096 x 4096:
+// 17.8 / 19.2), beyond that with eight waves and two workgroups a compute unit (4096 x 2048 x 1024: 11.9 us, four waves 16.0);
+// 256x256 from a full round on (4096 x 4096 x 1024: 17.4 us, 128x128 21.8).  Tiles of 128x64 and 256x128 in their rounds: no
+// more than 5 % ahead of the square ones (2048 x 1024 x 4096: 12.8 us) or behind (4096 x 4096 x 4096: 49.9 us, 256x256 39.7).
 static int pick_tile(const MxGemmParams& p, hipStream_t stream) {
-  if (p.M <= 32) return launch_tile<1, 4, 32, 64, 4, true>(p, stream);
-  const auto tiles = [&](int64_t e) { return (p.M + e - 1) / e * ((p.N + e - 1) / e); };
-  if (tiles(64) <= 512 || p.M <= 64 || p.N <= 64) return launch_tile<2, 2, 64, 64, 4, true>(p, stream);
-  if (tiles(128) <= 256) return launch_tile<2, 2, 128, 128, 3, false>(p, stream);
-  if (tiles(256) < 256) return launch_tile<2, 4, 128, 128, 2, false>(p, stream);
+  const auto tiles = [&](int64_t i, int64_t j) { return (p.M + i - 1) / i * ((p.N + j - 1) / j); };
+  if (p.M <= 32 || tiles(32, 64) <= 256) return launch_tile<1, 4, 32, 64, 4, true>(p, stream);
+  if (tiles(64, 64) <= 512 || p.M <= 64 || p.N <= 64) return launch_tile<2, 2, 64, 64, 4, true>(p, stream);
+  if (tiles(128, 128) <= 256) return launch_tile<2, 2, 128, 128, 3, false>(p, stream);
+  if (tiles(256, 256) < 256) return launch_tile<2, 4, 128, 128, 2, false>(p, stream);
   return launch_tile<4, 2, 256, 256, 2, false>(p, stream);
 }
 
@@ -309,8 +311,8 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
     p.as = (const unsigned char*)a_scales;
   }
   // Blocks of 16 rows of B times runs of 16 (up to 16 rows of A) or 32 tokens.  Above 16 rows the few-rows kernel is ahead
-  // while they are at most two rounds of the compute units (512 x 512 x 4096: 7.6 us, 64x64 tiles 9.0; 64 x 4096 x 4096: 7.6 / 8.9;
-  // 100 x 4096 x 4096, four rounds: 10.6 / 8.9); the tiled kernels' offsets inside a tile have 32 bits.
+  // while one round takes its blocks (24 x 2048 x 4096: 5.5 us, 32x64 tiles 6.8; 512 x 512 x 4096, two rounds: 7.4 / 6.9);
+  // the tiled kernels' offsets inside a tile have 32 bits.
   const int64_t blocks = (d->N + 15) / 16 * (d->M <= 16 ? 1 : (d->M + 31) / 32);
   if (src == SRC_F32) {
     rc = pick_fused<SRC_F32>(p, blocks, stream);
@@ -322,8 +324,6 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
     rc = pick_fused<SRC_MX>(p, blocks, stream);
   } else if (blocks <= 256 || p.steps >= 1 << 16) {
     rc = launch_few<SRC_MX, 1, 2>(p, stream);
-  } else if (blocks <= 512) {
-    rc = launch_few<SRC_MX, 2, 2>(p, stream);
   } else {
     rc = pick_tile(p, stream);
   }

@@ -3,7 +3,7 @@
 // Block tile BI x BJ, K step 256 elements = 128 bytes of every row.  LDS holds NS stages of codes (rows of
 // eight 16-byte chunks, XOR-swizzled by row, the swizzle applied on the global side) and two spans of
 // scales (32 bytes a row: four K steps).  Both travel by direct copies (global_load_lds, 16 bytes a
-// lane; 4 for scales that are not 16-byte aligned).  A K step is two matrix instructions deep and runs in four phases (half of
+// lane; scale rows begin at any word, and rows of fewer than 16 bytes come by words).  A K step is two matrix instructions deep and runs in four phases (half of
 // the wave tile's rows, sub-step); the fragments of a phase are read while the one before multiplies.
 // The one barrier of a step stands in front of its last phase, where all reads of the stage are
 // issued; the copies of the step NS later start behind it, spread over three phases.  A fragment is
@@ -23,7 +23,7 @@ namespace amos {
 struct MxTileParams {
   MxGemmParams g;
   int tiles_i, tiles_j;
-  int vec_scales;       // rows of scales are whole 16-byte pieces from 16-byte aligned memory on
+  int vec_scales;       // a row of scales has 16 bytes
   int stream_out;       // an fp32 C larger than the L2s together: written past them (8192^3: 281 -> 270 us)
 };
 
@@ -87,7 +87,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   };
   // Scales: a row's 32 bytes of four K steps at once (8 bytes a row and step would touch as many memory lines per
   // step as the codes do).  Bit 3 of the row swaps the two 16-byte halves of its place: sixteen rows on different
-  // banks.  What lies behind a row's end is fetched from its last bytes (and not used).
+  // banks.  A row whose length is no multiple of 16 ends in its last 16 bytes once more: scale_at() reads that much
+  // further on.
   auto scale_row = [&](int row) -> unsigned {   // row of the tile (A's, then B's) -> row of its operand, from the tile's first on
     return (unsigned)(row < BI ? (bi0 + row < p.M ? row : p.M - 1 - bi0) : (bj0 + row - BI < p.N ? row - BI : p.N - 1 - bj0));
   };
@@ -101,29 +102,22 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     const unsigned char* const sb = first < BI ? asbase : bsbase;
     asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds0 + SCALES + (span & 1) * SPAN + first * 32), "v"(off), "s"(sb) : "memory");
   };
-  auto scale_word = [&](int span, int u) {     // 8 rows, eight lanes a row
+  auto scale_word = [&](int u) {               // 8 rows, eight lanes a row (the words behind its end: the last one, not used)
     const int first = (wave + NW * u) * 8, row = first + (lane >> 3);
-    const int want = span * 8 + ((lane & 7) ^ (((row >> 3) & 1) << 2));
+    const int want = (lane & 7) ^ (((row >> 3) & 1) << 2);
     const unsigned r = scale_row(row);
     const int last = p.steps - 1;
     const unsigned off = r * (unsigned)spitch + (unsigned)(want < last ? want : last) * 4;
     const unsigned char* const sb = first < BI ? asbase : bsbase;
-    asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds0 + SCALES + (span & 1) * SPAN + first * 32), "v"(off), "s"(sb) : "memory");
+    asm volatile("s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" ::"s"(lds0 + SCALES + first * 32), "v"(off), "s"(sb) : "memory");
   };
-  // step kt's share of the next span's scales (in the first two steps of a span: what follows them until their use is
-  // more than the waits below leave in flight)
+  // the next span's scales, in the first step of a span: the copies that follow them until their use are more than the
+  // waits below leave in flight.  (A second span has rows of 32 bytes and more behind it.)
   auto issue_scales = [&](int kt) {
     const int span = (kt >> 2) + 1;
-    if (span * 4 >= KT || (kt & 2)) return;
-    if (t.vec_scales) {
-      if ((kt & 1) == 0)
+    if (span * 4 >= KT || (kt & 3)) return;
 #pragma unroll
-        for (int u = 0; u < SV; ++u) scale_vec(span, u);
-    } else {
-#pragma unroll
-      for (int u = 0; u < (SW + 1) / 2; ++u)
-        if ((kt & 1) * ((SW + 1) / 2) + u < SW) scale_word(span, (kt & 1) * ((SW + 1) / 2) + u);
-    }
+    for (int u = 0; u < SV; ++u) scale_vec(span, u);
   };
 
   // Which of a K step's eight blocks a lane group takes is free as long as both operands agree: group q takes blocks
@@ -134,7 +128,10 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   const int swap = ((frag_row >> 3) & 1) * 16;
   const int as_off = arow * 32 + 2 * frag_q + swap, bs_off = (BI + brow) * 32 + 2 * frag_q + swap;
   // LDS address of step kt's scale bytes for a row whose place is `off`
-  auto scale_at = [&](int off, int kt) { return smem + SCALES + ((kt >> 2) & 1) * SPAN + (off ^ (((kt >> 1) & 1) * 16)) + (kt & 1) * 8; };
+  auto scale_at = [&](int off, int kt, bool used) {
+    const int ahead = t.vec_scales && used ? (kt >> 1) * 16 + 16 - (int)spitch : 0;   // the last 16 bytes begin earlier by so much
+    return smem + SCALES + ((kt >> 2) & 1) * SPAN + (off ^ (((kt >> 1) & 1) * 16)) + (kt & 1) * 8 + (ahead > 0 ? ahead : 0);
+  };
 
   v4f acc[TI][TJ];
 #pragma unroll
@@ -150,7 +147,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
       for (int u = 0; u < SV; ++u) scale_vec(0, u);
     } else {
 #pragma unroll
-      for (int u = 0; u < SW; ++u) scale_word(0, u);
+      for (int u = 0; u < SW; ++u) scale_word(u);
     }
   };
   int st = 0;   // this step's stage
@@ -161,7 +158,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     int xa[2][TI], xb[2][TJ];
     auto read_all = [&](int kt, int stage, auto set) {
       const char* s = smem + stage * STAGE;
-      const char *sa = scale_at(as_off, kt), *sb = scale_at(bs_off, kt);
+      const char *sa = scale_at(as_off, kt, kt < full), *sb = scale_at(bs_off, kt, kt < full);
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
 #pragma unroll
@@ -177,10 +174,9 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     auto step = [&](int kt, auto set, auto other) {
       const int next = st + 1 == NS ? 0 : st + 1, after = kt + NS < KT ? kt + NS : KT - 1;
       // this wave's copies of the next step have landed (those of the NS - 2 steps behind it may be under way; copies of
-      // one width complete in their order, for scales by words all are waited for once a span) and its reads of this
-      // one too: behind the barrier the next stage is whole and this one is free
-      if (NS > 2 && (t.vec_scales || (kt & 3) != 3)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      // one width complete in their order) and its reads of this one too: behind the barrier the next stage is whole and
+      // this one is free
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
       asm volatile("s_barrier" ::: "memory");
       read_all(kt + 1, next, other);   // (behind the last step: read and not used)
       __builtin_amdgcn_sched_barrier(0);
@@ -219,7 +215,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     int ax[TI], bx[TJ], bx_next[TJ];   // scales: a register serves both sub-steps
     auto read_a = [&](int kt, int stage, auto h, auto ks) {
       const char* s = smem + stage * STAGE;
-      const char* x = scale_at(as_off, kt);
+      const char* x = scale_at(as_off, kt, kt < full);
 #pragma unroll
       for (int a = 0; a < HA; ++a) {
         af[h][a] = *(const mx_v4i*)(s + (a_off ^ (ks * 16)) + (h * HA + a) * 2048);
@@ -228,7 +224,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     };
     auto read_b = [&](int kt, int stage, auto ks, int* to) {
       const char* s = smem + stage * STAGE;
-      const char* x = scale_at(bs_off, kt);
+      const char* x = scale_at(bs_off, kt, kt < full);
 #pragma unroll
       for (int b = 0; b < TJ; ++b) {
         bf[ks][b] = *(const mx_v4i*)(s + (b_off ^ (ks * 16)) + b * 2048);
@@ -266,7 +262,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     }
 #pragma unroll
     for (int u = 0; u < FIRST; ++u) issue_copy(NS - 1 < KT ? NS - 1 : KT - 1, NS - 1, u);
-    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * CH + FIRST) : "memory");
+    if (t.vec_scales) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * CH + FIRST) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     read_a(0, 0, I0, I0);
     read_b(0, 0, I0, bx);
 
@@ -284,9 +281,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
       phase(I0, I1, -1, 0, 0);
       // all reads of this stage are issued; once they and this wave's copies of the next step are done (those of the NS - 2
       // steps behind it may be under way), meet: behind the barrier the next stage is whole and this one is free.  (Copies
-      // of one width complete in their order; for scales by words all are waited for once a span.)
-      if (NS > 2 && (t.vec_scales || (kt & 3) != 3)) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
-      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      // of one width complete in their order.)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
       asm volatile("s_barrier" ::: "memory");
       read_a(kt + 1, next, I0, I0);   // (behind the last step: read and not used)
       read_b(kt + 1, next, I0, bx_next);
@@ -300,7 +296,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   if (half) {   // four blocks, one for each lane group
     const char* s = smem + st * STAGE;
     const int ah = mx_lds_offset(arow, frag_q), bh = OPER + mx_lds_offset(brow, frag_q);
-    const char *axh = scale_at(as_off - frag_q, full), *bxh = scale_at(bs_off - frag_q, full);   // (byte q, not 2q)
+    const char *axh = scale_at(as_off - frag_q, full, true), *bxh = scale_at(bs_off - frag_q, full, true);   // (byte q, not 2q)
     mx_v4i g[TJ];
     int y[TJ];
 #pragma unroll
