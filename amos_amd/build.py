@@ -1,4 +1,4 @@
-"""Builds libamos_mi355x.so for gfx950 with hipcc:  python -m amos_amd.build"""
+"""Builds libamos_mi355x.so for gfx950 with hipcc, and _calls.so beside it:  python -m amos_amd.build"""
 import os
 import subprocess
 import sys
@@ -7,6 +7,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libamos_mi355x.so")
+CALLS = os.path.join(HERE, "_calls.so")
 
 # -packed-fp32-ops is switched off: the compiler must not form v_pk_*_f32
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature",
@@ -21,6 +22,22 @@ def sources():
     hip = sorted(f for f in os.listdir(CSRC) if f.endswith(".hip"))
     cpp = sorted(f for f in os.listdir(CSRC) if f.endswith(".cpp"))
     return [os.path.join(CSRC, f) for f in hip + cpp]
+
+
+def build_calls(verbose=True):
+    """the native calls of ops.py: host code against this PyTorch's headers"""
+    import sysconfig
+
+    import torch
+    base = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I" + os.path.join(ROOT, "include"),
+           "-isystem", os.path.join(base, "include"), "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
+           "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "python", "calls.cc"),
+           "-L" + os.path.join(base, "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-o", CALLS]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.check_call(cmd)
 
 
 def build(verbose=True, jobs=8):
@@ -84,6 +101,7 @@ def build(verbose=True, jobs=8):
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
+    build_calls(verbose)
     return OUT
 
 

@@ -539,17 +539,27 @@ def _like_check(what, t, shape, device):
         raise ValueError("%s must be of shape %s on %s, got %s on %s" % (what, tuple(shape), device, tuple(t.shape), t.device))
 
 
-class _Plans(dict):
-    """what follows from a call's shapes and types alone (checked descriptor, workspace bytes), by these"""
+class _Native(object):
+    """The entry points below in their common form (contiguous tensors on the current device, its current stream) as
+    native calls, csrc/python/calls.cc: each returns None for a call that it does not take, and the call is then made,
+    or refused, the long way.  Group norm with its statistics, 1 x 7 x 7 x 512: 6.6 us a call; checked and allocated in the interpreter, 11.1."""
 
-    def keep(self, key, plan):
-        if len(self) >= 4096:
-            self.clear()
-        self[key] = plan
-        return plan
+    def __getattr__(self, name):   # (the first call: a missing build is an error)
+        lib = _lib.load()
+        try:
+            from . import _calls
+        except ImportError as e:
+            raise RuntimeError("amos_amd/_calls.so is missing or does not fit this PyTorch: build it with `python -m amos_amd.build`") from e
+        _calls.setup(Mxfp4, _current_device, _raw_stream,
+                     *(ctypes.cast(f, ctypes.c_void_p).value for f in (
+                         lib.amos_mxfp4_quantize, lib.amos_mxfp4_dequantize, lib.amos_mxfp4_gemm, lib.amos_mxfp4_gemm_workspace_bytes,
+                         lib.amos_group_norm, lib.amos_group_norm_backward, lib.amos_group_norm_workspace_bytes)))
+        for f in ("quantize", "dequantize", "gemm", "group_norm", "group_norm_backward"):
+            setattr(self, f, getattr(_calls, f))
+        return object.__getattribute__(self, name)
 
 
-_MX_PLANS, _MX_GEMM_PLANS, _NORM_PLANS = _Plans(), _Plans(), _Plans()
+_native = _Native()
 
 
 def mxfp4_quantize(x, axis=1, out=None, stream=None):
@@ -558,14 +568,14 @@ def mxfp4_quantize(x, axis=1, out=None, stream=None):
     product that sums over the rows of x takes.  A block's scale brings its largest magnitude into
     [4, 8); elements are rounded to nearest even and saturate at 6; a block with an infinity or a NaN
     stands for NaN."""
+    if stream is None:
+        done = _native.quantize(x, axis, out)
+        if done is not None:
+            return done
     _need_device(x)
-    key = (x.shape, x.dtype, axis)
-    plan = _MX_PLANS.get(key) or _MX_PLANS.keep(key, _quantize_plan(*key))
+    plan = _quantize_plan(x.shape, x.dtype, axis)
     if out is not None and (not isinstance(out, Mxfp4) or out.shape != plan[1] or out.device != x.device):
         raise ValueError("out must be an Mxfp4 of shape %s on %s, got %r" % (plan[1], x.device, out))
-    index = x.get_device()
-    if stream is None and index == _current_device():
-        return _quantize(_raw_stream(index), plan, x, out)
     return _on(_quantize, x.device, stream, plan, x, out)
 
 
@@ -592,15 +602,16 @@ def _quantize(s, plan, x, out):
 
 def mxfp4_dequantize(q, dtype=torch.float32, out=None, stream=None):
     """the values an Mxfp4 stands for, rounded once to `dtype` (fp32 and bf16 hold them all)"""
+    if stream is None:
+        done = _native.dequantize(q, dtype, out)
+        if done is not None:
+            return done
     if not isinstance(q, Mxfp4):
         raise ValueError("q must be an Mxfp4, got %s" % type(q))
     if out is not None:
         _need_device(out)
         _check_out(out, q.shape, dtype, q.codes)
     d = _lib.Mxfp4Desc(q.shape[0], q.shape[1], _float_code("the result", dtype), 1)
-    index = q.codes.get_device()
-    if stream is None and index == _current_device():
-        return _dequantize(_raw_stream(index), q, d, dtype, out)
     return _on(_dequantize, q.codes.device, stream, q, d, dtype, out)
 
 
@@ -615,6 +626,10 @@ def mxfp4_gemm(a, b, out=None, out_dtype=torch.float32, add=None, bias=None, str
     """C[M,N] = sum_k A(m,k) B(n,k) (+ bias[N]) (+ add[M,N]); b is an Mxfp4 of shape (N, K), a an
     Mxfp4 of shape (M, K) or a dense matrix [M, K] (fp32, fp16, bf16) that the call quantises the way
     mxfp4_quantize does.  fp32 accumulation, one rounding to the output's type; `add` may be `out`."""
+    if stream is None:
+        done = _native.gemm(a, b, out, out_dtype, add, bias)
+        if done is not None:
+            return done
     if not isinstance(b, Mxfp4):
         raise ValueError("b must be an Mxfp4, got %s" % type(b))
     device = b.codes.device
@@ -625,8 +640,7 @@ def mxfp4_gemm(a, b, out=None, out_dtype=torch.float32, add=None, bias=None, str
         raise ValueError("a is on %s, b on %s" % (a.device, device))
     if out is not None:
         out_dtype = out.dtype
-    key = (a.shape, b.shape, a.dtype if dense else None, out_dtype)
-    plan = _MX_GEMM_PLANS.get(key) or _MX_GEMM_PLANS.keep(key, _mxfp4_gemm_plan(*key))
+    plan = _mxfp4_gemm_plan(a.shape, b.shape, a.dtype if dense else None, out_dtype)
     if out is not None:
         _like_check("out", out, plan[1], device)
     epi = None
@@ -639,9 +653,6 @@ def mxfp4_gemm(a, b, out=None, out_dtype=torch.float32, add=None, bias=None, str
             _like_check("the added operand", add, plan[1], device)
             epi.add, epi.add_dtype = add.data_ptr(), _float_code("the added operand", add.dtype)
         epi = ctypes.byref(epi)
-    index = device.index
-    if stream is None and index == _current_device():
-        return _mxfp4_gemm(_raw_stream(index), plan, a, b, dense, out, out_dtype, epi)
     return _on(_mxfp4_gemm, device, stream, plan, a, b, dense, out, out_dtype, epi)
 
 
@@ -693,11 +704,10 @@ def _group_norm_plan(gradient, x_shape, x_dtype, y_dtype, groups, weight_dtype, 
     return ctypes.byref(d), need, (ext["c"],), (ext["n"], groups)
 
 
-def _group_norm_key(gradient, x, y_dtype, groups, weight, bias, eps, activation, layout):
+def _group_norm_checked(gradient, x, y_dtype, groups, weight, bias, eps, activation, layout):
     """the plan of a call, its coefficients checked"""
-    key = (gradient, x.shape, x.dtype, y_dtype, groups, None if weight is None else weight.dtype, None if bias is None else bias.dtype, eps,
-           activation, layout)
-    plan = _NORM_PLANS.get(key) or _NORM_PLANS.keep(key, _group_norm_plan(*key))
+    plan = _group_norm_plan(gradient, x.shape, x.dtype, y_dtype, groups, None if weight is None else weight.dtype,
+                            None if bias is None else bias.dtype, eps, activation, layout)
     device = x.device
     if weight is not None:
         _like_check("weight", weight, plan[2], device)
@@ -717,6 +727,10 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, lay
     then None / 'relu' / 'silu'.  Statistics and arithmetic are fp32, the result is x's type or
     out_dtype (a convolution's fp32 output can leave at 16 bits for the next one); `out` may be x.
     stats=True: (y, mean, rstd), both fp32 [N, groups], for group_norm_backward."""
+    if stream is None:
+        done = _native.group_norm(x, groups, weight, bias, eps, activation, layout, out_dtype, out, stats)
+        if done is not None:
+            return done
     _need_device(x)
     if out is not None:
         _like_check("out", out, x.shape, x.device)
@@ -725,10 +739,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, lay
         out_dtype = out.dtype
     elif out_dtype is None:
         out_dtype = x.dtype
-    plan = _group_norm_key(False, x, out_dtype, groups, weight, bias, eps, activation, layout)
-    index = x.get_device()
-    if stream is None and index == _current_device():
-        return _group_norm(_raw_stream(index), plan, x, weight, bias, out, out_dtype, stats)
+    plan = _group_norm_checked(False, x, out_dtype, groups, weight, bias, eps, activation, layout)
     return _on(_group_norm, x.device, stream, plan, x, weight, bias, out, out_dtype, stats)
 
 
@@ -747,16 +758,17 @@ def _group_norm(s, plan, x, weight, bias, out, out_dtype, stats):
 def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, activation=None, layout="nhwc", stream=None):
     """gradients of group_norm: (dx of x's type, dweight, dbias in fp32 -- None where the coefficient
     is), from the statistics that group_norm(..., stats=True) returned for x"""
+    if stream is None:
+        done = _native.group_norm_backward(dy, x, mean, rstd, groups, weight, bias, activation, layout)
+        if done is not None:
+            return done
     _need_device(dy, x, mean, rstd)
     if dy.shape != x.shape or dy.device != x.device:
         raise ValueError("dy is %s on %s, x %s on %s" % (tuple(dy.shape), dy.device, tuple(x.shape), x.device))
-    plan = _group_norm_key(True, x, dy.dtype, groups, weight, bias, 0.0, activation, layout)
+    plan = _group_norm_checked(True, x, dy.dtype, groups, weight, bias, 0.0, activation, layout)
     for what, t in (("mean", mean), ("rstd", rstd)):
         if t.shape != plan[3] or t.device != x.device or t.dtype != torch.float32:
             raise ValueError("%s must be fp32 of shape %s on %s, got %s %s on %s" % (what, plan[3], x.device, t.dtype, tuple(t.shape), t.device))
-    index = x.get_device()
-    if stream is None and index == _current_device():
-        return _group_norm_backward(_raw_stream(index), plan, dy, x, mean, rstd, weight, bias)
     return _on(_group_norm_backward, x.device, stream, plan, dy, x, mean, rstd, weight, bias)
 
 
