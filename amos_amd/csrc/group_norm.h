@@ -154,10 +154,10 @@ __device__ __forceinline__ GnSlab gn_slab(const GnParams& p, int vec) {
   return w;
 }
 // Sums over each group of a slab: the threads' values `v` (one each for UNI, else one for each channel) meet in
-// `lds` ([rows][entries]), a team of lanes adds a group's, in an order that does not depend on timing; totals in
-// `total` [groups].  Barriers in front, between and behind.
-template <int VEC, bool UNI>
-__device__ __forceinline__ void gn_group_sums(const GnParams& p, const GnSlab& w, const float* v, float* lds, float* total) {
+// `lds` ([rows][entries]), a team of lanes adds a group's, in an order that does not depend on timing; `of` each
+// sum in `total` [groups].  Barriers between and behind.
+template <int VEC, bool UNI, class F>
+__device__ __forceinline__ void gn_group_sums(const GnParams& p, const GnSlab& w, const float* v, float* lds, float* total, F of) {
   const int per = UNI ? p.cols : p.cols * VEC;
   const int epg = per / w.groups;
   if (w.active) {
@@ -172,12 +172,18 @@ __device__ __forceinline__ void gn_group_sums(const GnParams& p, const GnSlab& w
   const int lane = threadIdx.x & (team - 1), step = (int)blockDim.x / team, entries = p.rows * epg;
   for (int g = threadIdx.x / team; g < w.groups; g += step) {
     float s = 0.f;
-    for (int e = lane; e < entries; e += team) {
-      const int r = fast_div(e, p.by_epg);
-      s += lds[r * per + g * epg + (e - r * epg)];
+    for (int e = lane; e < entries; e += 4 * team) {   // four reads in flight
+      float x[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int at = e + u * team, r = fast_div(at, p.by_epg);
+        x[u] = at < entries ? lds[r * per + g * epg + (at - r * epg)] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += x[u];
     }
     s = gn_team_sum(s, team);
-    if (lane == 0) total[g] = s;
+    if (lane == 0) total[g] = of(s);
   }
   __syncthreads();
 }

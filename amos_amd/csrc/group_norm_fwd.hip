@@ -205,10 +205,10 @@ __global__ __launch_bounds__(1024) void amos_gn_held(const GnParams p) {
       }
     }
   }
-  gn_group_sums<VEC, UNI>(p, w, s, lds, total);
+  gn_group_sums<VEC, UNI>(p, w, s, lds, total, [&](float sum) { return sum / count; });
 #pragma unroll
   for (int i = 0; i < S; ++i) {
-    mean[i] = total[group[i]] / count;
+    mean[i] = total[group[i]];
     s[i] = 0.f;
   }
   if (w.active) {
@@ -225,9 +225,9 @@ __global__ __launch_bounds__(1024) void amos_gn_held(const GnParams p) {
       }
     }
   }
-  gn_group_sums<VEC, UNI>(p, w, s, lds, total + w.groups);
+  gn_group_sums<VEC, UNI>(p, w, s, lds, total + w.groups, [&](float sum) { return 1.f / sqrtf(sum / count + p.eps); });
 #pragma unroll
-  for (int i = 0; i < S; ++i) rstd[i] = 1.f / sqrtf(total[w.groups + group[i]] / count + p.eps);
+  for (int i = 0; i < S; ++i) rstd[i] = total[w.groups + group[i]];
   if (!w.active) return;
   if (w.row == 0) {   // a group's first lane and channel
 #pragma unroll
