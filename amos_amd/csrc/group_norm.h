@@ -7,10 +7,13 @@
 //     dweight[c] = sum d h,  dbias[c] = sum d      (over images and pixels)
 //     dx = (d weight - E[d weight] - h E[d weight h]) / sqrt(var + eps)   (E over the group)
 //
-// Both move bytes: a launch reads the tensors once for the sums, a second one reads them again and
-// writes.  A workgroup takes a run of pixels ("chunk") and a tile of channels; a lane keeps VEC
-// neighbouring channels and strides over pixels, so that a wave's loads are whole rows.  Sums are
+// Both move bytes.  Where whole groups of an image fit into a workgroup's registers, one launch reads
+// the tensors once and writes ("held"); else a launch reads them for the sums and a second one
+// reads them again and writes.  There a workgroup takes a run of pixels ("chunk") and a tile of channels; a
+// lane keeps VEC neighbouring channels and strides over pixels, so that a wave's loads are whole rows.  Sums are
 // joined in a fixed order (no atomics: the same bits on every run).
+// 16 x 128 x 128 x 256 bf16 in two launches: forward 91 us, 4.4 TB/s over its three passes (a large copy: 5.1), gradient
+// 145 us, 4.6 TB/s over five; 1 x 128 x 128 x 512: 19 and 23 us (with tiles of all channels, 128 workgroups: 36 and 41).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -31,6 +31,9 @@ struct GnChannels {
   }
 };
 
+// 32 x 56 x 56 x 256 bf16 (154 MB in and out): 25 + 28 us with inputs from memory, 21 + 28 us where they are still in the
+// last cache.  One launch that holds x and dy of an image's groups in registers and LDS (512 threads, 25 vectors each)
+// needs 48 - 52 us and 5 for the coefficients: it reads less, but its reads, arithmetic and writes follow one another.
 // ---- first launch: sums of d and d h over a chunk, by channel and (with the weights) by group -------
 template <class XT, class YT, int VEC, bool SILU>
 __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_partial(const GnParams p) {

@@ -59,43 +59,56 @@ inline bool gn_plan_held(const amos_group_norm_desc_t* d, bool gradient, int vec
 // The two-launch plan; 1: this vector length does not divide the tiles
 inline int gn_plan_tiles(const amos_group_norm_desc_t* d, bool gradient, int vec, GnParams& p, GnPlan& plan) {
   const int64_t most = (int64_t)kGnThreads * vec;   // channels a workgroup can lay side by side
-  const int64_t C = d->C, cpg = C / d->groups;
-  int64_t ct, tiles, sub = 1;
+  const int64_t C = d->C, cpg = C / d->groups, P = p.P;
   if (C % vec) return 1;
-  if (C <= most) {
-    ct = C;
-    tiles = 1;
-  } else if (cpg <= most) {            // whole groups, and whole vectors
+  // chunks: some 1024 workgroups, each thread at least four pixels, at most 128 partial results to join
+  const auto lay = [&](int64_t ct, int64_t tiles) {
+    p.ct = (int)ct;
+    p.tiles = (int)tiles;
+    p.cols = (int)((ct + vec - 1) / vec);
+    p.rows = kGnThreads / p.cols;
+    int64_t chunks = 1024 / (d->N * tiles);
+    chunks = chunks < 1 ? 1 : chunks > 128 ? 128 : chunks;
+    int64_t chunk = (P + chunks - 1) / chunks;
+    if (chunk < 4 * p.rows) chunk = 4 * p.rows;
+    if (chunk > P) chunk = P;
+    p.chunk = (int)chunk;
+    p.chunks = (int)((P + chunk - 1) / chunk);
+    return p.N * tiles * p.chunks;   // workgroups
+  };
+  int64_t sub = 1;
+  if (cpg <= most) {            // tiles of whole groups, and whole vectors
     int64_t unit = 1;
     while (unit * cpg % vec) ++unit;
-    const int64_t per_tile = most / cpg / unit * unit;
+    const auto tiles_of = [&](int64_t per_tile) { return (d->groups + per_tile - 1) / per_tile; };
+    int64_t per_tile = C <= most ? d->groups : most / cpg / unit * unit;
     if (per_tile == 0) return 1;
-    ct = per_tile * cpg;
-    tiles = (d->groups + per_tile - 1) / per_tile;
-  } else {                             // several tiles a group
+    if (tiles_of(per_tile) > 65535) return set_error(AMOS_ERR_UNSUPPORTED, "group norm of %lld channels in %d groups", (long long)C, d->groups);
+    int64_t now = lay(per_tile * cpg, tiles_of(per_tile));
+    // few images: narrower tiles, down to a memory line of a pixel, as long as that makes more workgroups (each joins the
+    // partial results of fewer groups then, too)
+    while (now < 1024) {
+      const int64_t next = (per_tile / 2 + unit - 1) / unit * unit;
+      if (next == 0 || next >= per_tile || next * cpg * dense_size(d->x_dtype) < 128) break;
+      const int64_t then = lay(next * cpg, tiles_of(next));
+      if (then <= now) {
+        lay(per_tile * cpg, tiles_of(per_tile));
+        break;
+      }
+      now = then;
+      per_tile = next;
+    }
+  } else {                      // several tiles a group
     if (cpg % vec) return 1;
     sub = (cpg + most - 1) / most;
-    ct = ((cpg + sub - 1) / sub + vec - 1) / vec * vec;
+    const int64_t ct = ((cpg + sub - 1) / sub + vec - 1) / vec * vec;
     sub = (cpg + ct - 1) / ct;
-    tiles = d->groups * sub;
+    if (d->groups * sub > 65535) return set_error(AMOS_ERR_UNSUPPORTED, "group norm of %lld channels in %d groups", (long long)C, d->groups);
+    lay(ct, d->groups * sub);
   }
-  if (tiles > 65535) return set_error(AMOS_ERR_UNSUPPORTED, "group norm of %lld channels in %d groups", (long long)C, d->groups);
   plan.vec = vec;
   plan.held = 0;
-  p.ct = (int)ct;
-  p.tiles = (int)tiles;
   p.sub = (int)sub;
-  p.cols = (int)((ct + vec - 1) / vec);
-  p.rows = kGnThreads / p.cols;
-  // chunks: some 1024 workgroups, each thread at least four pixels, at most 128 partial results to join
-  const int64_t P = p.P;
-  int64_t chunks = 1024 / (d->N * tiles);
-  chunks = chunks < 1 ? 1 : chunks > 128 ? 128 : chunks;
-  int64_t chunk = (P + chunks - 1) / chunks;
-  if (chunk < 4 * p.rows) chunk = 4 * p.rows;
-  if (chunk > P) chunk = P;
-  p.chunk = (int)chunk;
-  p.chunks = (int)((P + chunk - 1) / chunk);
   if (((int64_t)p.N * p.chunks + C / 16 + 1) * kGnThreads >= kGnGridThreads) return set_error(AMOS_ERR_UNSUPPORTED, "group norm of %d images", p.N);
   p.slots = p.chunks * p.sub;
   p.by_cols = make_fast_div((uint32_t)p.cols);

@@ -15,7 +15,8 @@ namespace amos {
 // to 16 TT tokens; its waves take K in turns of 512 elements (four instructions' worth: 256 contiguous
 // bytes of every row), and there are as many waves, up to 16, as give each one turn: all of a wave's loads
 // are in flight together.  A row's scales of a turn are one 16-byte load.  The waves' sums meet in LDS,
-// added in the order of the waves.
+// added in the order of the waves.  1 x 4096 x 4096 (8.9 MB of weights) 5.4 us, 1 x 16384 x 4096 (36 MB) 9.0 us = 4.0 TB/s;
+// a launch that does nothing takes some 2.5 us of that.
 // SRC: what A is -- codes, or (fp32 / fp16 / bf16) elements that are quantised here: a lane's fragment
 // is exactly one block, so it finds the block's scale without any exchange.
 enum { SRC_MX = 0, SRC_F32 = 1, SRC_F16 = 2, SRC_BF16 = 3 };

@@ -9,6 +9,14 @@
 // issued; the copies of the step NS later start behind it, spread over three phases.  A fragment is
 // one 16-byte LDS read; its block's scale is a byte of a register that a 2-byte read fills for both
 // sub-steps and that the matrix instruction takes as it is: no instruction touches a scale.
+// (FLAT: small wave tiles read a whole step's fragments at once, a step ahead.)
+//
+// 8192^3, fp32 out: 300 us = 3.7 PFLOP/s.  Its matrix instructions alone take 164 us (7.2 PFLOP/s is what they reach on
+// random operands), with their LDS reads 198 - 203, the copies alone 147 (64 KB a K step and compute unit at 28 bytes a
+// cycle, a fifth of it from behind the L2), everything but the stores 238: neither is at its limit by itself (matrix
+// cores 42 % busy, LDS 30 %), the two waves of a SIMD do not fill each other's waits.  The 268 MB of results take the rest.
+// Tried there: four waves of 128x128 (370 us: one wave a SIMD cannot hide its copies), waves as 2x4 (290 where 4x2
+// took 277), stores straight from the registers (301 / 281), copies in two phases (319 / 277).
 // Rows past M / N repeat the last one (their sums are not stored).  K is padded to 128 by the format; an
 // odd number of 128s ends in a half step whose second half is neither read from memory (its lanes fetch
 // the first half again: the row may be the buffer's last) nor multiplied.

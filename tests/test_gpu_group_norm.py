@@ -75,7 +75,8 @@ SHAPES = [("nhwc", (1, 1, 1, 1), 1), ("nhwc", (2, 1, 1, 64), 4), ("nhwc", (1, 7,
           ("nhwc", (2, 5, 3, 7), 7), ("nhwc", (2, 33, 31, 48), 16), ("nhwc", (1, 64, 65, 8), 8), ("nhwc", (2, 56, 56, 64), 32),
           ("nhwc", (2, 6, 5, 2304), 32), ("nhwc", (1, 4, 9, 4100), 1), ("nhwc", (2, 3, 3, 2500), 5), ("nhwc", (1, 3, 5, 6144), 2),
           ("nhwc", (5, 9, 8, 40), 5), ("ndhwc", (2, 3, 5, 7, 24), 3), ("hwnc", (9, 8, 3, 64), 16), ("dhwnc", (2, 4, 5, 3, 33), 11),
-          ("nhwc", (2, 128, 130, 16), 2), ("hwnc", (40, 41, 6, 128), 4), ("nhwc", (8, 40, 40, 64), 8)]
+          ("nhwc", (2, 128, 130, 16), 2), ("hwnc", (40, 41, 6, 128), 4), ("nhwc", (8, 40, 40, 64), 8), ("nhwc", (1, 70, 66, 512), 32),
+          ("nhwc", (2, 71, 67, 360), 15), ("hwnc", (67, 71, 1, 330), 11), ("nhwc", (1, 66, 65, 4224), 3)]
 
 
 @pytest.mark.parametrize("layout, shape, groups", SHAPES)
