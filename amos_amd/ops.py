@@ -757,7 +757,8 @@ def _group_norm(s, plan, x, weight, bias, out, out_dtype, stats):
 
 def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, activation=None, layout="nhwc", stream=None):
     """gradients of group_norm: (dx of x's type, dweight, dbias in fp32 -- None where the coefficient
-    is), from the statistics that group_norm(..., stats=True) returned for x"""
+    is), from the statistics that group_norm(..., stats=True) returned for x (rstd below 2^63: its square
+    is formed in fp32)"""
     if stream is None:
         done = _native.group_norm_backward(dy, x, mean, rstd, groups, weight, bias, activation, layout)
         if done is not None:

@@ -425,7 +425,7 @@ int amos_mxfp4_gemm(const amos_mxfp4_gemm_desc_t* desc, const amos_mxfp4_epilogu
  * are fp32; mean and rstd = 1 / sqrt(var + eps) are written as fp32 [N][groups] where not NULL.  y may
  * be x where their types agree.
  * Gradient (with the forward's mean and rstd): dx of x's type, dweight and dbias fp32 [C] or NULL; dy has
- * y's type.  dx may be dy or x where the types agree.  Results do not depend on the order in which
+ * y's type.  dx may be dy or x where the types agree.  rstd^2 is formed in fp32: rstd below 2^63.  Results do not depend on the order in which
  * workgroups run.
  * The reference leaves normalisation layers to its fallback scheduler
  * (python/tvm/tensor_graph/core/auto_schedule/auto_schedule.py:1090-1160).
