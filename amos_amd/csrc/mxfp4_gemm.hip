@@ -219,20 +219,34 @@ static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
   return 0;
 }
 
-// The tile, by how many there are: 32x64 up to 32 rows of A (24 x 10240 x 8192: 12.6 us, 64x64 15.1, the few-rows kernel
-// 15.5) and while one round of the compute units takes them (333 x 1000 x 2050: 5.4 us, 64x64 6.2; 64 x 8192 x 4096, 256 tiles:
-// 7.5 / 8.7; 1000 x 1000 x 2048, 512: 6.4 / 6.2); 64x64 (two workgroups a compute unit) while one round takes
-// them or one side has no more rows (2048 x 1024 x 4096: 12.4 us, 128x128 17.3; 4096 x 1024 x 2048, 1024 of them: 15.6 / 11.5);
-// 128x128 in one round with four waves and three stages (4096 x 1024 x 2048: 11.5 us, eight waves 11.6; 1024 x 4096 x 4096:
-// 17.8 / 19.2), beyond that with eight waves and two workgroups a compute unit (4096 x 2048 x 1024: 11.9 us, four waves 16.0);
-// 256x256 from a full round on (4096 x 4096 x 1024: 17.4 us, 128x128 21.8).  Tiles of 128x64 and 256x128 in their rounds: no
-// more than 5 % ahead of the square ones (2048 x 1024 x 4096: 12.8 us) or behind (4096 x 4096 x 4096: 49.9 us, 256x256 39.7).
+// The tile: the one whose rounds of the 256 compute units take the least time.  `one`, `two`: microseconds of a round with
+// one and with two workgroups a unit (the larger tiles' LDS leaves room for one), all at K = 4096; at other K the ratios
+// hold well enough (over 45 shapes of 32 to 8200 rows, 64 to 11000 columns, K 280 to 7700: at most 11 % behind the best of the five, 1 % on the mean).
+//   2048 x 2048 x 2048: 128x128 10.6 us, 64x64 14.5, 256x256 19.6      4096 x 2048 x 4096: 128x256 24.1 us, 128x128 31.8, 256x256 33.1
+//   333 x 1000 x 2050: 32x64 5.4 us, 64x64 6.1                         3000 x 3000 x 1000: 256x256 15.0 us, 128x256 18.4, 128x128 19.4
+// Four stages and a step's fragments read at once let 128x128 in one round wait for neither memory nor LDS (1024 x 4096 x 4096:
+// 15.7 us; three stages with phases 20.3, two workgroups a unit with two stages 19.9).
+struct TileCost {
+  int bi, bj;
+  double one, two;
+};
+constexpr TileCost kTiles[] = {{32, 64, 7.0, 9.4}, {64, 64, 8.6, 12.3}, {128, 128, 16.0, 32.0}, {128, 256, 24.1, 48.2}, {256, 256, 38.5, 77.0}};
 static int pick_tile(const MxGemmParams& p, hipStream_t stream) {
-  const auto tiles = [&](int64_t i, int64_t j) { return (p.M + i - 1) / i * ((p.N + j - 1) / j); };
-  if (p.M <= 32 || tiles(32, 64) <= 256) return launch_tile<1, 4, 32, 64, 4, true>(p, stream);
-  if (tiles(64, 64) <= 512 || p.M <= 64 || p.N <= 64) return launch_tile<2, 2, 64, 64, 4, true>(p, stream);
-  if (tiles(128, 128) <= 256) return launch_tile<2, 2, 128, 128, 3, false>(p, stream);
-  if (tiles(256, 256) < 256) return launch_tile<2, 4, 128, 128, 2, false>(p, stream);
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < 5; ++i) {
+    const TileCost& t = kTiles[i];
+    const int64_t n = (int64_t)((p.M + t.bi - 1) / t.bi) * ((p.N + t.bj - 1) / t.bj), rest = n % 512;
+    const double cost = (double)(n / 512) * t.two + (rest > 256 ? t.two : rest ? t.one : 0.0);
+    if (i == 0 || cost < least) {
+      best = i;
+      least = cost;
+    }
+  }
+  if (p.M <= 32 || best == 0) return launch_tile<1, 4, 32, 64, 4, true>(p, stream);
+  if (best == 1) return launch_tile<2, 2, 64, 64, 4, true>(p, stream);
+  if (best == 2) return launch_tile<2, 4, 128, 128, 4, true>(p, stream);
+  if (best == 3) return launch_tile<2, 4, 128, 256, 2, true>(p, stream);
   return launch_tile<4, 2, 256, 256, 2, false>(p, stream);
 }
 

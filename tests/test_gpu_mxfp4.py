@@ -120,7 +120,7 @@ def test_unaligned_storage_and_outputs(gpu, dtype):
 PRODUCTS = [(1, 1, 1), (1, 17, 33), (1, 1000, 4096), (2, 130, 640), (5, 64, 129), (16, 16, 128), (17, 48, 384), (24, 257, 1000),
             (33, 31, 2050), (64, 64, 256), (65, 100, 511), (100, 300, 513), (127, 129, 128), (128, 128, 1024), (130, 260, 640),
             (255, 257, 1152), (256, 256, 512), (300, 520, 2304), (512, 384, 768), (513, 1023, 96), (1025, 70, 4352), (700, 1300, 32), (40, 4500, 900),
-            (300, 9000, 200), (24, 8300, 700), (9, 12400, 1100), (31, 8290, 1536), (1500, 1700, 1152), (1530, 1666, 1024), (2310, 2250, 640), (2304, 2304, 512), (520, 1100, 2700), (60, 17000, 1200), (1000, 700, 4480), (4100, 4097, 384), (4096, 4098, 512)]
+            (300, 9000, 200), (24, 8300, 700), (9, 12400, 1100), (31, 8290, 1536), (1500, 1700, 1152), (1530, 1666, 1024), (2310, 2250, 640), (2304, 2304, 512), (520, 1100, 2700), (60, 17000, 1200), (1000, 700, 4480), (3100, 3005, 1100), (3005, 3100, 512), (3000, 2900, 300), (4100, 4097, 384), (4096, 4098, 512)]
 
 
 @pytest.mark.parametrize("out", DTYPES)
