@@ -9,7 +9,8 @@
 // issued; the copies of the step NS later start behind it, spread over three phases.  A fragment is
 // one 16-byte LDS read; its block's scale is a byte of a register that a 2-byte read fills for both
 // sub-steps and that the matrix instruction takes as it is: no instruction touches a scale.
-// (FLAT: small wave tiles read a whole step's fragments at once, a step ahead.)
+// FLAT, where two sets of a step's fragments fit into the registers (all but 256x256): they are read at once, a step ahead
+// (2048 x 2048 x 8192, 128x128 tiles with four stages: 26.7 us; in phases with two or three 34).
 //
 // 8192^3, fp32 out: 300 us = 3.7 PFLOP/s.  Its matrix instructions alone take 164 us (7.2 PFLOP/s is what they reach on
 // random operands), with their LDS reads 198 - 203, the copies alone 147 (64 KB a K step and compute unit at 28 bytes a
@@ -160,8 +161,8 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
   };
   int st = 0;   // this step's stage
   if constexpr (FLAT) {
-    // Small wave tiles have too few matrix instructions a phase to hide an LDS read behind: all fragments of a step are
-    // read at once, a step ahead, into a second set of registers.
+    // All fragments of a step are read at once, a step ahead, into a second set of registers: what hides an LDS read
+    // is a step's matrix instructions, not a phase's.
     mx_v4i fa[2][2][TI], fb[2][2][TJ];
     int xa[2][TI], xb[2][TJ];
     auto read_all = [&](int kt, int stage, auto set) {

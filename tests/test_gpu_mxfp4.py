@@ -267,6 +267,23 @@ def test_more_than_32_bits_of_elements(gpu):
     assert big.shape == (1 << 20, 64) and not big.codes.any() and not big.scales.any()
 
 
+@pytest.mark.parametrize("M, N", [(9, 20), (70, 1100)])
+def test_very_long_sums(gpu, M, N):
+    """K past what the tiles' 32-bit offsets reach: zeros but for its first and last elements"""
+    from amos_amd import ops
+    K, ends = (1 << 23) + 300, 520
+    g = torch.Generator().manual_seed(M)
+    parts = []
+    for rows in (M, N):
+        c = torch.randint(0, 16, (rows, 2 * ends), generator=g)
+        packed = torch.zeros(rows, ref.pitch(K), dtype=torch.uint8)
+        packed[:, :ends // 2] = (c[:, 0:ends:2] + 16 * c[:, 1:ends:2]).to(torch.uint8)
+        packed[:, (K - ends) // 2:K // 2] = (c[:, ends::2] + 16 * c[:, ends + 1::2]).to(torch.uint8)
+        parts.append((ops.Mxfp4(packed.cuda(), torch.full((rows, ref.pitch(K) // 16), 127, dtype=torch.uint8, device="cuda"), K), ref.GRID[c]))
+    want = parts[0][1] @ parts[1][1].t()        # multiples of 1/4 below 2^17: exact
+    assert torch.equal(ops.mxfp4_gemm(parts[0][0], parts[1][0]).cpu(), want.float())
+
+
 def test_columns_in_several_launches(gpu):
     """axis 0 of a matrix wider than one launch takes"""
     from amos_amd import ops
