@@ -266,11 +266,16 @@ static int check_desc(const amos_mxfp4_gemm_desc_t* d) {
 
 static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
-// Dense rows of A are quantised by the few-rows kernel itself where every workgroup can afford to read all of them:
-// up to four rows their bytes are fewer than those of the sixteen rows of B that it reads anyway.  More: by a
-// launch of its own, codes and scales in the workspace.
-constexpr int kFusedRows = 4;
-static bool quantize_first(const amos_mxfp4_gemm_desc_t* d) { return d->a_dtype != AMOS_MXFP4 && d->M > kFusedRows; }
+// Dense rows of A are quantised by the few-rows kernel itself where every workgroup can afford to read and convert all of
+// them: one turn of K a wave, at most 32 KB, no more than three rounds of workgroups.  Else by a launch of its own, codes
+// and scales in the workspace.  (On the GPU, fused / apart: 1 x 4096 x 4096 bf16 5.9 / 5.9 us, 8 x 4096 x 2048 4.7 / 5.3,
+// 16 x 1024 x 1024 4.4 / 5.0; 1 x 4096 x 8192 9.3 / 8.5, 4 x 4096 x 4096 fp32, 64 KB, 6.8 / 6.2, 1 x 28672 x 8192 54 / 28.  A launch
+// and an allocation less are 3 us of the host's time as well.)
+static bool quantize_first(const amos_mxfp4_gemm_desc_t* d) {
+  if (d->a_dtype == AMOS_MXFP4) return false;
+  const bool fused = d->M <= 16 && d->K <= 4096 && d->N <= 768 * 16 && d->M * d->K * dense_size(d->a_dtype) <= 32 << 10;
+  return !fused;
+}
 
 static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, const void* A, const void* a_scales, const void* B,
                const void* b_scales, void* C, void* workspace, size_t ws_bytes, hipStream_t stream) {

@@ -155,7 +155,8 @@ def test_product_scales(gpu, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("M, N, K", [(1, 17, 33), (1, 1000, 4096), (3, 40, 200), (4, 64, 1024), (7, 33, 2050), (16, 50, 999), (24, 257, 1000), (100, 300, 520), (300, 520, 2304)])
+@pytest.mark.parametrize("M, N, K", [(1, 17, 33), (1, 1000, 4096), (3, 40, 200), (4, 64, 1024), (7, 33, 2050), (16, 50, 999), (24, 257, 1000), (100, 300, 520), (300, 520, 2304),
+                                     (2, 5000, 600), (8, 12200, 300), (16, 40, 1024), (3, 13000, 700), (1, 100, 5000)])
 def test_dense_rows_are_quantised_as_mxfp4_quantize_does(gpu, dtype, M, N, K):
     from amos_amd import ops
     a = awkward(M, K, dtype, M).cuda()
