@@ -140,6 +140,17 @@ PyObject* wrap_mx(const Mx& q) {
   return o;
 }
 
+// rows(codes, scales, cols): how many rows a matrix of these tensors has
+PyObject* rows_of(PyObject* const* a) {
+  Where w;
+  const at::Tensor &codes = tensor(a[0], w), &scales = tensor(a[1], w);
+  const int64_t cols = integer(a[2]), pitch = cols < 1 ? 0 : (cols + 127) / 128 * 64;
+  if (!pitch || codes.scalar_type() != at::kByte || scales.scalar_type() != at::kByte || codes.dim() != 2 || scales.dim() != 2 || codes.size(0) < 1 ||
+      codes.size(1) != pitch || scales.size(0) != codes.size(0) || scales.size(1) != pitch / 16)
+    throw NotTaken();
+  return PyLong_FromLongLong(codes.size(0));
+}
+
 // quantize(x, axis, out)
 PyObject* quantize(PyObject* const* a) {
   Where w;
@@ -399,6 +410,7 @@ PyMethodDef method(const char* name, const char* doc) {
 }
 PyMethodDef methods[] = {
     {"setup", setup, METH_VARARGS, "setup(Mxfp4, current device, current stream, seven addresses)"},
+    method<rows_of, 3>("rows", "rows(codes, scales, cols)"),
     method<quantize, 3>("quantize", "quantize(x, axis, out)"),
     method<dequantize, 3>("dequantize", "dequantize(q, dtype, out)"),
     method<gemm, 6>("gemm", "gemm(a, b, out, out_dtype, add, bias)"),

@@ -471,6 +471,10 @@ class Mxfp4(object):
     __slots__ = ("codes", "scales", "shape")
 
     def __init__(self, codes, scales, cols):
+        rows = _native.rows(codes, scales, cols)
+        if rows is not None:
+            self.codes, self.scales, self.shape = codes, scales, (rows, cols)
+            return
         _need_device(codes, scales)
         pitch = mxfp4_pitch(cols)
         rows = codes.shape[0] if codes.dim() == 2 else 0
@@ -554,7 +558,7 @@ class _Native(object):
                      *(ctypes.cast(f, ctypes.c_void_p).value for f in (
                          lib.amos_mxfp4_quantize, lib.amos_mxfp4_dequantize, lib.amos_mxfp4_gemm, lib.amos_mxfp4_gemm_workspace_bytes,
                          lib.amos_group_norm, lib.amos_group_norm_backward, lib.amos_group_norm_workspace_bytes)))
-        for f in ("quantize", "dequantize", "gemm", "group_norm", "group_norm_backward"):
+        for f in ("rows", "quantize", "dequantize", "gemm", "group_norm", "group_norm_backward"):
             setattr(self, f, getattr(_calls, f))
         return object.__getattribute__(self, name)
 
