@@ -51,6 +51,13 @@ struct GnParams {
   int y_dtype;
 };
 
+// 1 / sqrt(var + eps).  Sums are fp32: a variance that left their range (deviations from some 2^64 / sqrt(elements of the
+// group) up) is no variance, and its group's results are NaN, not the bias that a factor of 1 / infinity would leave
+__device__ __forceinline__ float gn_rstd(float var, float eps) {
+  const float v = var + eps;
+  return v < __builtin_inff() ? 1.f / sqrtf(v) : __builtin_nanf("");
+}
+
 // 1 / (1 + exp(-z)), from z times -log2(e)
 __device__ __forceinline__ float gn_sigmoid2(float scaled) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(scaled)); }
 constexpr float kGnLog2e = 1.44269504088896341f;

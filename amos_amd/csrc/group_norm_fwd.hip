@@ -102,7 +102,7 @@ __device__ __forceinline__ void gn_join(const GnParams& p, int n, int g, int lan
     d += at[e * 3 + 2] + at[e * 3] * off * off;
   }
   const float var = gn_team_sum(d, team) / total;
-  rstd = 1.f / sqrtf(var + p.eps);
+  rstd = gn_rstd(var, p.eps);
 }
 
 // ---- second launch: normalise, scale, activate ----------------------------------------------------
@@ -227,7 +227,7 @@ __global__ __launch_bounds__(1024) void amos_gn_held(const GnParams p) {
       }
     }
   }
-  gn_group_sums<VEC, UNI>(p, w, s, lds, total + w.groups, [&](float sum) { return 1.f / sqrtf(sum / count + p.eps); });
+  gn_group_sums<VEC, UNI>(p, w, s, lds, total + w.groups, [&](float sum) { return gn_rstd(sum / count, p.eps); });
 #pragma unroll
   for (int i = 0; i < S; ++i) rstd[i] = total[w.groups + group[i]];
   if (!w.active) return;

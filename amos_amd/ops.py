@@ -729,7 +729,9 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, lay
     """act(group norm of x) over a channels-last tensor (layout nhwc, ndhwc, hwnc or dhwnc): per image
     and group of neighbouring channels h = (x - mean) / sqrt(var + eps), then h * weight[C] + bias[C],
     then None / 'relu' / 'silu'.  Statistics and arithmetic are fp32, the result is x's type or
-    out_dtype (a convolution's fp32 output can leave at 16 bits for the next one); `out` may be x.
+    out_dtype (a convolution's fp32 output can leave at 16 bits for the next one); `out` may be x.  A group
+    whose values or squared deviations add up to 2^128 and more (deviations from about 2^64 / sqrt(elements
+    of the group) up), or that holds an infinity or a NaN, is NaN.
     stats=True: (y, mean, rstd), both fp32 [N, groups], for group_norm_backward."""
     if stream is None:
         done = _native.group_norm(x, groups, weight, bias, eps, activation, layout, out_dtype, out, stats)

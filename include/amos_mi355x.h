@@ -422,8 +422,10 @@ int amos_mxfp4_gemm(const amos_mxfp4_gemm_desc_t* desc, const amos_mxfp4_epilogu
  *   mean = E[x], var = E[(x - mean)^2], h = (x - mean) / sqrt(var + eps), y = act(h weight[c] + bias[c])
  * x, y (dy, dx) are dense in one of the channels-last layouts of the convolutions (AMOS_LAYOUT_NHWC,
  * AMOS_LAYOUT_HWNC); weight, bias [C] of one type, or NULL (ones, zeros).  Arithmetic and statistics
- * are fp32; mean and rstd = 1 / sqrt(var + eps) are written as fp32 [N][groups] where not NULL.  y may
- * be x where their types agree.
+ * are fp32; mean and rstd = 1 / sqrt(var + eps) are written as fp32 [N][groups] where not NULL.  A group
+ * whose values or squared deviations add up to 2^128 and more (deviations from about 2^64 / sqrt(elements
+ * of the group) up), or that holds an infinity or a NaN, has rstd and results of NaN.  y may be x where
+ * their types agree.
  * Gradient (with the forward's mean and rstd): dx of x's type, dweight and dbias fp32 [C] or NULL; dy has
  * y's type.  dx may be dy or x where the types agree.  rstd^2 is formed in fp32: rstd below 2^63.  Results do not depend on the order in which
  * workgroups run.
