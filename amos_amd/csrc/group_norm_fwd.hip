@@ -17,7 +17,8 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_partial(const GnParams p) 
     float cnt = 0.f;
     int q = w.p0 + w.row;
     constexpr int B = 4;
-    // four pixels at a time: their own mean and deviations, joined to the running ones
+    // four pixels at a time: their own mean and deviations, joined to the running ones (delta times delta times `both` in this
+    // order: in front of the first pixels `both` is 0 and delta the mean itself, whose square fp32 need not hold)
     for (; q + (B - 1) * p.rows < w.p1; q += B * p.rows) {
       float v[B][VEC];
 #pragma unroll
@@ -33,7 +34,7 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_partial(const GnParams p) 
         for (int b = 0; b < B; ++b) d2 += (v[b][i] - s) * (v[b][i] - s);
         const float delta = s - mean[i];
         mean[i] += delta * share;
-        m2[i] += d2 + delta * delta * both;
+        m2[i] += d2 + delta * (delta * both);
       }
       cnt += B;
     }
@@ -45,7 +46,7 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_partial(const GnParams p) 
       for (int i = 0; i < VEC; ++i) {
         const float delta = v[i] - mean[i];
         mean[i] += delta * share;
-        m2[i] += delta * delta * both;
+        m2[i] += delta * (delta * both);
       }
       cnt += 1.f;
     }

@@ -37,3 +37,14 @@ def test_sums_inside_the_range(gpu, shape, power):
     """values of 2^40 (squares of 2^80 times some 2^20 elements) and of 2^-70 (squares of 2^-140 beside eps): the formula's"""
     w, b = coefficients(shape[-1], 4)
     check_forward(make("nhwc", shape, 3) * 2.0 ** power, 2, w, b, "silu", "nhwc", torch.float32)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("value", [2.0 ** 70, -2.0 ** 90])
+def test_large_equal_values(gpu, shape, value):
+    """a mean whose square fp32 does not hold, and no deviation: h is 0, whichever kernel runs"""
+    from amos_amd import ops
+    w, b = (t.cuda() for t in coefficients(shape[-1], 4))
+    y, mean, rstd = ops.group_norm(torch.full(shape, value, device="cuda"), 2, w, b, stats=True)
+    assert (mean == value).all() and torch.allclose(rstd, torch.full_like(rstd, 1e-5 ** -0.5), rtol=1e-6)
+    assert torch.equal(y, b.expand(shape))
