@@ -11,7 +11,8 @@ static int run_gradient(const amos_group_norm_desc_t* d, const void* dy, const v
                         const float* rstd, void* dx, float* dweight, float* dbias, void* workspace, size_t ws_bytes, hipStream_t stream) {
   GnParams p;
   GnPlan plan;
-  int rc = gn_check(d, {dy, x, dx}, weight, bias, p);
+  if (!d) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
+  int rc = gn_check(d, {{dy, d->y_dtype}, {x, d->x_dtype}, {dx, d->x_dtype}}, weight, bias, {mean, rstd, dweight, dbias}, p);
   if (rc) return rc;
   if (!mean || !rstd) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
   rc = gn_choose(d, true, p, plan);

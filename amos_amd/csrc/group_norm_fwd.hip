@@ -294,7 +294,8 @@ static int run_forward(const amos_group_norm_desc_t* d, const void* x, const voi
                        void* workspace, size_t ws_bytes, hipStream_t stream) {
   GnParams p;
   GnPlan plan;
-  int rc = gn_check(d, {x, y}, weight, bias, p);
+  if (!d) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
+  int rc = gn_check(d, {{x, d->x_dtype}, {y, d->y_dtype}}, weight, bias, {mean, rstd}, p);
   if (rc == 0) rc = gn_choose(d, false, p, plan);
   if (rc == 0) rc = gn_workspace(plan, p, workspace, ws_bytes);
   if (rc) return rc;

@@ -127,10 +127,16 @@ inline int gn_choose(const amos_group_norm_desc_t* d, bool gradient, GnParams& p
   return rc;
 }
 
-inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<const void*> tensors, const void* weight, const void* bias, GnParams& p) {
+struct GnTensor {
+  const void* at;
+  int dtype;
+};
+// `tensors`: the dense ones; `vectors`: fp32 statistics and gradients, or null
+inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<GnTensor> tensors, const void* weight, const void* bias,
+                    std::initializer_list<const void*> vectors, GnParams& p) {
   if (!d) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
-  for (const void* t : tensors)
-    if (!t) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
+  for (const GnTensor& t : tensors)
+    if (!t.at) return set_error(AMOS_ERR_BAD_ARG, "null pointer argument");
   memset(&p, 0, sizeof(p));
   if (d->N < 1 || d->C < 1 || d->D < 1 || d->H < 1 || d->W < 1)
     return set_error(AMOS_ERR_BAD_ARG, "group norm of extents N %lld, D %lld, H %lld, W %lld, C %lld", (long long)d->N, (long long)d->D,
@@ -162,9 +168,12 @@ inline int gn_check(const amos_group_norm_desc_t* d, std::initializer_list<const
   p.y_dtype = d->y_dtype;
   p.weight = weight;
   p.bias = bias;
-  const int es = dense_size(d->x_dtype) < dense_size(d->y_dtype) ? dense_size(d->x_dtype) : dense_size(d->y_dtype);
-  for (const void* t : tensors)
-    if ((uintptr_t)t & (es - 1)) return set_error(AMOS_ERR_BAD_ARG, "group norm: misaligned tensor");
+  for (const GnTensor& t : tensors)
+    if ((uintptr_t)t.at & (dense_size(t.dtype) - 1)) return set_error(AMOS_ERR_BAD_ARG, "group norm: misaligned tensor");
+  for (const void* t : {weight, bias})
+    if (t && ((uintptr_t)t & (dense_size(d->affine_dtype) - 1))) return set_error(AMOS_ERR_BAD_ARG, "group norm: misaligned weight or bias");
+  for (const void* t : vectors)
+    if ((uintptr_t)t & 3) return set_error(AMOS_ERR_BAD_ARG, "group norm: misaligned statistics or gradients of the coefficients");
   return 0;
 }
 
@@ -172,7 +181,7 @@ inline size_t gn_plan_bytes(const GnPlan& plan) { return (size_t)((plan.part_flo
 inline size_t gn_workspace_bytes(const amos_group_norm_desc_t* d, bool gradient) {
   GnParams p;
   GnPlan plan;
-  if (gn_check(d, {}, nullptr, nullptr, p) || gn_choose(d, gradient, p, plan)) return 0;
+  if (gn_check(d, {}, nullptr, nullptr, {}, p) || gn_choose(d, gradient, p, plan)) return 0;
   return gn_plan_bytes(plan);
 }
 
