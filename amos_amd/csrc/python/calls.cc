@@ -117,9 +117,11 @@ Mx unpack(PyObject* o, Where& w) {
   Py_XDECREF(shape);
   PyErr_Clear();
   const int64_t pitch = (q.cols + 127) / 128 * 64;
-  if (!ok || q.rows < 1 || q.cols < 1 || !q.codes.is_cuda() || !q.scales.is_cuda() || q.codes.numel() != q.rows * pitch ||
-      q.scales.numel() != q.rows * (pitch / 16) || !q.codes.is_contiguous() || !q.scales.is_contiguous())
-    throw NotTaken();
+  if (!ok || q.rows < 1 || q.cols < 1) throw NotTaken();
+  const auto is = [&](const at::Tensor& t, int64_t wide) {
+    return t.is_cuda() && t.scalar_type() == at::kByte && t.dim() == 2 && t.size(0) == q.rows && t.size(1) == wide && t.is_contiguous();
+  };
+  if (!is(q.codes, pitch) || !is(q.scales, pitch / 16)) throw NotTaken();
   if (w.device < 0) w.device = q.codes.get_device();
   if (q.codes.get_device() != w.device || q.scales.get_device() != w.device) throw NotTaken();
   return q;

@@ -495,6 +495,20 @@ class Mxfp4(object):
         return "Mxfp4(shape=%s, device=%s)" % (self.shape, self.device)
 
 
+def _mx_check(what, q):
+    """an Mxfp4 whose attributes still fit each other (they can be set), contiguous and on one device"""
+    if not isinstance(q, Mxfp4):
+        raise ValueError("%s must be an Mxfp4, got %s" % (what, type(q)))
+    rows, cols = q.shape
+    pitch = mxfp4_pitch(cols)
+    _need_device(q.codes, q.scales)
+    for t, wide in ((q.codes, pitch), (q.scales, pitch // 16)):
+        if t.dtype is not torch.uint8 or t.shape != (rows, wide) or t.device != q.codes.device:
+            raise ValueError("%s of shape %s wants uint8 codes [%d, %d] and scales [%d, %d] on one device, got %s %s on %s and %s %s on %s"
+                             % (what, (rows, cols), rows, pitch, rows, pitch // 16, q.codes.dtype, tuple(q.codes.shape), q.codes.device,
+                                q.scales.dtype, tuple(q.scales.shape), q.scales.device))
+
+
 def mxfp4_pitch(cols):
     """bytes of a row of codes"""
     if cols < 1:
@@ -578,8 +592,10 @@ def mxfp4_quantize(x, axis=1, out=None, stream=None):
             return done
     _need_device(x)
     plan = _quantize_plan(x.shape, x.dtype, axis)
-    if out is not None and (not isinstance(out, Mxfp4) or out.shape != plan[1] or out.device != x.device):
-        raise ValueError("out must be an Mxfp4 of shape %s on %s, got %r" % (plan[1], x.device, out))
+    if out is not None:
+        _mx_check("out", out)
+        if out.shape != plan[1] or out.device != x.device:
+            raise ValueError("out must be an Mxfp4 of shape %s on %s, got %r" % (plan[1], x.device, out))
     return _on(_quantize, x.device, stream, plan, x, out)
 
 
@@ -610,8 +626,7 @@ def mxfp4_dequantize(q, dtype=torch.float32, out=None, stream=None):
         done = _native.dequantize(q, dtype, out)
         if done is not None:
             return done
-    if not isinstance(q, Mxfp4):
-        raise ValueError("q must be an Mxfp4, got %s" % type(q))
+    _mx_check("q", q)
     if out is not None:
         _need_device(out)
         _check_out(out, q.shape, dtype, q.codes)
@@ -634,12 +649,13 @@ def mxfp4_gemm(a, b, out=None, out_dtype=torch.float32, add=None, bias=None, str
         done = _native.gemm(a, b, out, out_dtype, add, bias)
         if done is not None:
             return done
-    if not isinstance(b, Mxfp4):
-        raise ValueError("b must be an Mxfp4, got %s" % type(b))
+    _mx_check("b", b)
     device = b.codes.device
     dense = not isinstance(a, Mxfp4)
     if dense:
         _need_device(a)
+    else:
+        _mx_check("a", a)
     if a.device != device:
         raise ValueError("a is on %s, b on %s" % (a.device, device))
     if out is not None:
