@@ -1,4 +1,4 @@
-"""Builds libamos_mi355x.so for gfx950 with hipcc, and _calls.so beside it:  python -m amos_amd.build"""
+"""Builds libamos_mi355x.so for gfx950 with hipcc, and, where PyTorch's headers are, _calls.so beside it:  python -m amos_amd.build"""
 import os
 import subprocess
 import sys
@@ -25,12 +25,24 @@ def sources():
 
 
 def build_calls(verbose=True):
-    """the native calls of ops.py: host code against this PyTorch's headers"""
+    """the native calls of ops.py: host code against this PyTorch's headers.  Without a PyTorch that has headers, or without
+    a host compiler, they are left out (the path is None then): ops.py makes its calls through ctypes"""
+    import shutil
     import sysconfig
-
-    import torch
+    if os.path.exists(CALLS):   # (of another PyTorch, perhaps)
+        os.remove(CALLS)
+    cxx = os.environ.get("CXX", "g++")
+    try:
+        import torch
+    except ImportError:
+        torch = None
+    lacks = ("PyTorch" if torch is None else "a host compiler (%s)" % cxx if shutil.which(cxx.split()[0]) is None else
+             "PyTorch's headers" if not os.path.isdir(os.path.join(os.path.dirname(torch.__file__), "include", "torch")) else None)
+    if lacks:
+        print("without _calls.so: %s is missing, amos_amd.ops calls through ctypes" % lacks, flush=True)
+        return None
     base = os.path.dirname(torch.__file__)
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    cmd = cxx.split() + ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            "-D_GLIBCXX_USE_CXX11_ABI=%d" % torch._C._GLIBCXX_USE_CXX11_ABI, "-I" + os.path.join(ROOT, "include"),
            "-isystem", os.path.join(base, "include"), "-isystem", os.path.join(base, "include", "torch", "csrc", "api", "include"),
            "-isystem", sysconfig.get_paths()["include"], os.path.join(CSRC, "python", "calls.cc"),
@@ -38,6 +50,7 @@ def build_calls(verbose=True):
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.check_call(cmd)
+    return CALLS
 
 
 def build(verbose=True, jobs=8):

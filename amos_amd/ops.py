@@ -5,6 +5,7 @@ computation goes through libamos_mi355x.so.  There is no CPU or eager fallback:
 tensors that are not on a HIP device are rejected.
 """
 import ctypes
+import os
 
 import torch
 
@@ -557,22 +558,33 @@ def _like_check(what, t, shape, device):
         raise ValueError("%s must be of shape %s on %s, got %s on %s" % (what, tuple(shape), device, tuple(t.shape), t.device))
 
 
+_CALLS_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_calls.so")
+
+
 class _Native(object):
     """The entry points below in their common form (contiguous tensors on the current device, its current stream) as
     native calls, csrc/python/calls.cc: each returns None for a call that it does not take, and the call is then made,
     or refused, the long way.  Group norm with its statistics, 1 x 7 x 7 x 512: 6.6 us a call; checked and allocated in the interpreter, 11.1."""
 
-    def __getattr__(self, name):   # (the first call: a missing build is an error)
+    NAMES = ("rows", "quantize", "dequantize", "gemm", "group_norm", "group_norm_backward")
+
+    def __getattr__(self, name):   # (the first call)
+        if name not in self.NAMES:
+            raise AttributeError(name)
         lib = _lib.load()
+        if not os.path.exists(_CALLS_PATH):   # (built without PyTorch's headers: everything goes the long way)
+            for f in self.NAMES:
+                setattr(self, f, lambda *args: None)
+            return object.__getattribute__(self, name)
         try:
             from . import _calls
         except ImportError as e:
-            raise RuntimeError("amos_amd/_calls.so is missing or does not fit this PyTorch: build it with `python -m amos_amd.build`") from e
+            raise RuntimeError("amos_amd/_calls.so does not fit this PyTorch: build it with `python -m amos_amd.build`") from e
         _calls.setup(Mxfp4, _current_device, _raw_stream,
                      *(ctypes.cast(f, ctypes.c_void_p).value for f in (
                          lib.amos_mxfp4_quantize, lib.amos_mxfp4_dequantize, lib.amos_mxfp4_gemm, lib.amos_mxfp4_gemm_workspace_bytes,
                          lib.amos_group_norm, lib.amos_group_norm_backward, lib.amos_group_norm_workspace_bytes)))
-        for f in ("rows", "quantize", "dequantize", "gemm", "group_norm", "group_norm_backward"):
+        for f in self.NAMES:
             setattr(self, f, getattr(_calls, f))
         return object.__getattribute__(self, name)
 
