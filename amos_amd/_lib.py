@@ -120,8 +120,8 @@ EXPORTS = [
     "amos_conv3d", "amos_conv2d_noalloc", "amos_conv_packed_weights_bytes", "amos_conv_pack_weights", "amos_run_fused", "amos_time", "amos_time_fused", "amos_gather", "amos_time_gather",
     "amos_eltwise", "amos_time_eltwise", "amos_kernel_name", "amos_match", "amos_enumerate_mappings",
     "amos_mfma_ceiling", "amos_mxfp4_pitch", "amos_mxfp4_quantize", "amos_mxfp4_dequantize",
-    "amos_mxfp4_gemm_workspace_bytes", "amos_mxfp4_gemm", "amos_group_norm_workspace_bytes", "amos_group_norm",
-    "amos_group_norm_backward",
+    "amos_mxfp4_gemm_workspace_bytes", "amos_mxfp4_gemm_kernel_name", "amos_mxfp4_gemm",
+    "amos_group_norm_workspace_bytes", "amos_group_norm", "amos_group_norm_backward",
 ]
 
 _lib = None
@@ -191,6 +191,8 @@ def load():
     lib.amos_mxfp4_dequantize.argtypes = [ctypes.POINTER(Mxfp4Desc), vp, vp, vp, vp]
     lib.amos_mxfp4_gemm_workspace_bytes.argtypes = [ctypes.POINTER(Mxfp4GemmDesc)]
     lib.amos_mxfp4_gemm_workspace_bytes.restype = sz
+    lib.amos_mxfp4_gemm_kernel_name.argtypes = [ctypes.POINTER(Mxfp4GemmDesc)]
+    lib.amos_mxfp4_gemm_kernel_name.restype = ctypes.c_char_p
     lib.amos_mxfp4_gemm.argtypes = [ctypes.POINTER(Mxfp4GemmDesc), ctypes.POINTER(Mxfp4Epilogue), vp, vp, vp, vp, vp,
                                     vp, sz, vp]
     lib.amos_group_norm_workspace_bytes.argtypes = [ctypes.POINTER(GroupNormDesc), ctypes.c_int]

@@ -193,13 +193,6 @@ static int few_blocks(int64_t blocks) {
   const int64_t rt = (blocks + 255) / 256;
   return rt <= 3 ? (int)rt : 1;
 }
-template <int SRC>
-static int pick_fused(const MxGemmParams& p, int64_t blocks, hipStream_t stream) {
-  const int rt = few_blocks(blocks);
-  if (rt == 2) return launch_few<SRC, 2, 1>(p, stream);
-  if (rt == 3) return launch_few<SRC, 3, 1>(p, stream);
-  return launch_few<SRC, 1, 1>(p, stream);
-}
 
 // ---- many rows of A -----------------------------------------------------------------------------
 template <int WI, int WJ, int BI, int BJ, int NS, bool FLAT>
@@ -231,23 +224,19 @@ struct TileCost {
   double one, two;
 };
 constexpr TileCost kTiles[] = {{32, 64, 7.0, 9.4}, {64, 64, 8.6, 12.3}, {128, 128, 16.0, 32.0}, {128, 256, 24.1, 48.2}, {256, 256, 38.5, 77.0}};
-static int pick_tile(const MxGemmParams& p, hipStream_t stream) {
+static int pick_tile(int64_t M, int64_t N) {   // -> index
   int best = 0;
   double least = 0;
   for (int i = 0; i < 5; ++i) {
     const TileCost& t = kTiles[i];
-    const int64_t n = (int64_t)((p.M + t.bi - 1) / t.bi) * ((p.N + t.bj - 1) / t.bj), rest = n % 512;
+    const int64_t n = ((M + t.bi - 1) / t.bi) * ((N + t.bj - 1) / t.bj), rest = n % 512;
     const double cost = (double)(n / 512) * t.two + (rest > 256 ? t.two : rest ? t.one : 0.0);
     if (i == 0 || cost < least) {
       best = i;
       least = cost;
     }
   }
-  if (p.M <= 32 || best == 0) return launch_tile<1, 4, 32, 64, 4, true>(p, stream);
-  if (best == 1) return launch_tile<2, 2, 64, 64, 4, true>(p, stream);
-  if (best == 2) return launch_tile<2, 4, 128, 128, 4, true>(p, stream);
-  if (best == 3) return launch_tile<2, 4, 128, 256, 2, true>(p, stream);
-  return launch_tile<4, 2, 256, 256, 2, false>(p, stream);
+  return M <= 32 ? 0 : best;
 }
 
 int mx_quantize(const amos_mxfp4_desc_t* d, const void* x, void* codes, void* scales, hipStream_t stream);
@@ -275,6 +264,60 @@ static bool quantize_first(const amos_mxfp4_gemm_desc_t* d) {
   if (d->a_dtype == AMOS_MXFP4) return false;
   const bool fused = d->M <= 16 && d->K <= 4096 && d->N <= 768 * 16 && d->M * d->K * dense_size(d->a_dtype) <= 32 << 10;
   return !fused;
+}
+
+// Blocks of 16 rows of B times runs of 16 (up to 16 rows of A) or 32 tokens.  Above 16 rows the few-rows kernel is ahead
+// while one round takes its blocks (24 x 2048 x 4096: 5.5 us, 32x64 tiles 6.8; 512 x 512 x 4096, two rounds: 7.4 / 6.9);
+// the tiled kernels' offsets inside a tile have 32 bits.
+struct MxChoice {
+  int src;      // what the kernel reads A from (dense rows that are quantised first: SRC_MX)
+  int rt, tt;   // few rows: row blocks and token blocks of a workgroup; 0: tiles
+  int tile;     // ... of kTiles
+};
+static MxChoice choose(const amos_mxfp4_gemm_desc_t* d) {
+  MxChoice c = {SRC_MX, 0, 0, 0};
+  if (d->a_dtype != AMOS_MXFP4 && !quantize_first(d)) c.src = d->a_dtype == AMOS_F32 ? SRC_F32 : d->a_dtype == AMOS_F16 ? SRC_F16 : SRC_BF16;
+  const int64_t blocks = (d->N + 15) / 16 * (d->M <= 16 ? 1 : (d->M + 31) / 32);
+  const bool far = mx_pitch(d->K) / 64 >= 1 << 16;
+  if (c.src != SRC_MX || (d->M <= 16 && (blocks <= 768 || far))) {   // (16384 rows of B: 9.0 us, 32x64 tiles 8.3)
+    c.rt = few_blocks(blocks);
+    c.tt = 1;
+  } else if (blocks <= 256 || far) {
+    c.rt = 1;
+    c.tt = 2;
+  } else {
+    c.tile = pick_tile(d->M, d->N);
+  }
+  return c;
+}
+template <int SRC>
+static int launch_few_blocks(const MxGemmParams& p, int rt, hipStream_t stream) {
+  if (rt == 2) return launch_few<SRC, 2, 1>(p, stream);
+  if (rt == 3) return launch_few<SRC, 3, 1>(p, stream);
+  return launch_few<SRC, 1, 1>(p, stream);
+}
+static int launch_choice(const MxChoice& c, const MxGemmParams& p, hipStream_t stream) {
+  if (c.tt == 2) return launch_few<SRC_MX, 1, 2>(p, stream);
+  if (c.tt == 1) {
+    if (c.src == SRC_F32) return launch_few_blocks<SRC_F32>(p, c.rt, stream);
+    if (c.src == SRC_F16) return launch_few_blocks<SRC_F16>(p, c.rt, stream);
+    if (c.src == SRC_BF16) return launch_few_blocks<SRC_BF16>(p, c.rt, stream);
+    return launch_few_blocks<SRC_MX>(p, c.rt, stream);
+  }
+  if (c.tile == 0) return launch_tile<1, 4, 32, 64, 4, true>(p, stream);
+  if (c.tile == 1) return launch_tile<2, 2, 64, 64, 4, true>(p, stream);
+  if (c.tile == 2) return launch_tile<2, 4, 128, 128, 4, true>(p, stream);
+  if (c.tile == 3) return launch_tile<2, 4, 128, 256, 2, true>(p, stream);
+  return launch_tile<4, 2, 256, 256, 2, false>(p, stream);
+}
+static const char* choice_name(const MxChoice& c) {
+  static const char* const few[4][3] = {{"amos_mx_gemm_few<mxfp4,1,1>", "amos_mx_gemm_few<mxfp4,2,1>", "amos_mx_gemm_few<mxfp4,3,1>"},
+                                        {"amos_mx_gemm_few<f32,1,1>", "amos_mx_gemm_few<f32,2,1>", "amos_mx_gemm_few<f32,3,1>"},
+                                        {"amos_mx_gemm_few<f16,1,1>", "amos_mx_gemm_few<f16,2,1>", "amos_mx_gemm_few<f16,3,1>"},
+                                        {"amos_mx_gemm_few<bf16,1,1>", "amos_mx_gemm_few<bf16,2,1>", "amos_mx_gemm_few<bf16,3,1>"}};
+  static const char* const tile[5] = {"amos_mx_gemm_tile<32x64>", "amos_mx_gemm_tile<64x64>", "amos_mx_gemm_tile<128x128>",
+                                      "amos_mx_gemm_tile<128x256>", "amos_mx_gemm_tile<256x256>"};
+  return c.tt == 2 ? "amos_mx_gemm_few<mxfp4,1,2>" : c.tt == 1 ? few[c.src][c.rt - 1] : tile[c.tile];
 }
 
 static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, const void* A, const void* a_scales, const void* B,
@@ -307,11 +350,10 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
   p.K = (int)d->K;
   p.steps = (int)(mx_pitch(d->K) / 64);
   p.out_dtype = d->out_dtype;
-  int src = SRC_MX;
-  if (dense && !quantize_first(d)) {
+  const MxChoice c = choose(d);
+  if (c.src != SRC_MX) {
     p.dense = A;
-    src = d->a_dtype == AMOS_F32 ? SRC_F32 : d->a_dtype == AMOS_F16 ? SRC_F16 : SRC_BF16;
-  } else if (quantize_first(d)) {
+  } else if (dense) {
     const int64_t code_bytes = round256(d->M * mx_pitch(d->K));
     if (!workspace || ws_bytes < amos_mxfp4_gemm_workspace_bytes(d) || ((uintptr_t)workspace & 255))
       return set_error(AMOS_ERR_WORKSPACE, "4-bit product: %zu bytes of 256-byte aligned workspace wanted for A's codes", amos_mxfp4_gemm_workspace_bytes(d));
@@ -330,23 +372,7 @@ static int run(const amos_mxfp4_gemm_desc_t* d, const amos_mxfp4_epilogue_t* e, 
     p.a = (const unsigned char*)A;
     p.as = (const unsigned char*)a_scales;
   }
-  // Blocks of 16 rows of B times runs of 16 (up to 16 rows of A) or 32 tokens.  Above 16 rows the few-rows kernel is ahead
-  // while one round takes its blocks (24 x 2048 x 4096: 5.5 us, 32x64 tiles 6.8; 512 x 512 x 4096, two rounds: 7.4 / 6.9);
-  // the tiled kernels' offsets inside a tile have 32 bits.
-  const int64_t blocks = (d->N + 15) / 16 * (d->M <= 16 ? 1 : (d->M + 31) / 32);
-  if (src == SRC_F32) {
-    rc = pick_fused<SRC_F32>(p, blocks, stream);
-  } else if (src == SRC_F16) {
-    rc = pick_fused<SRC_F16>(p, blocks, stream);
-  } else if (src == SRC_BF16) {
-    rc = pick_fused<SRC_BF16>(p, blocks, stream);
-  } else if (d->M <= 16 && (blocks <= 768 || p.steps >= 1 << 16)) {   // (16384 rows of B: 9.0 us, 32x64 tiles 8.3)
-    rc = pick_fused<SRC_MX>(p, blocks, stream);
-  } else if (blocks <= 256 || p.steps >= 1 << 16) {
-    rc = launch_few<SRC_MX, 1, 2>(p, stream);
-  } else {
-    rc = pick_tile(p, stream);
-  }
+  rc = launch_choice(c, p, stream);
   if (rc) return rc;
   const hipError_t err = hipGetLastError();
   if (err != hipSuccess) return set_error(AMOS_ERR_HIP, "launch failed: %s", hipGetErrorString(err));
@@ -365,6 +391,8 @@ size_t amos_mxfp4_gemm_workspace_bytes(const amos_mxfp4_gemm_desc_t* desc) {
   const int64_t pitch = mx_pitch(desc->K);
   return (size_t)(round256(desc->M * pitch) + round256(desc->M * (pitch / 16)));
 }
+
+const char* amos_mxfp4_gemm_kernel_name(const amos_mxfp4_gemm_desc_t* desc) { return check_desc(desc) ? nullptr : choice_name(choose(desc)); }
 
 int amos_mxfp4_gemm(const amos_mxfp4_gemm_desc_t* desc, const amos_mxfp4_epilogue_t* epilogue, const void* A, const void* a_scales,
                     const void* B, const void* b_scales, void* C, void* workspace, size_t ws_bytes, void* stream) {

@@ -411,6 +411,9 @@ typedef struct {
 
 /* bytes of 256-byte aligned device scratch the call wants; less: AMOS_ERR_WORKSPACE */
 size_t amos_mxfp4_gemm_workspace_bytes(const amos_mxfp4_gemm_desc_t* desc);
+/* the kernel a product of these extents and types runs on, e.g. "amos_mx_gemm_tile<128x256>" (dense rows that it does not
+ * take itself are quantised by a launch in front of it); NULL where the call would be refused */
+const char* amos_mxfp4_gemm_kernel_name(const amos_mxfp4_gemm_desc_t* desc);
 int amos_mxfp4_gemm(const amos_mxfp4_gemm_desc_t* desc, const amos_mxfp4_epilogue_t* epilogue, const void* A,
                     const void* a_scales, const void* B, const void* b_scales, void* C, void* workspace,
                     size_t ws_bytes, void* stream);
