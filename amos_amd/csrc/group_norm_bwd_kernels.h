@@ -82,16 +82,16 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_partial(const GnP
   // ---- the pixel rows meet, in their order
   float* const cp = p.cpart + ((int64_t)blockIdx.x * p.C + w.c0) * 2;
   for (int c = threadIdx.x; c < w.width; c += kGnThreads) {
-    float a = 0.f, b = 0.f;
+    double a = 0., b = 0.;
     for (int r = 0; r < p.rows; ++r) {
       a += s1[r * p.cols * VEC + c];
       b += s2[r * p.cols * VEC + c];
     }
-    cp[c * 2] = a;
-    cp[c * 2 + 1] = b;
+    cp[c * 2] = (float)a;
+    cp[c * 2 + 1] = (float)b;
     const float weight = p.weight ? load_any(p.weight, w.c0 + c, p.affine_dtype) : 1.f;
-    s1[c] = a * weight;   // (row 0: read above by this thread only)
-    s2[c] = b * weight;
+    s1[c] = (float)a * weight;   // (row 0: read above by this thread only)
+    s2[c] = (float)b * weight;
   }
   __syncthreads();
   const int team = gn_team(w.groups), t = threadIdx.x, lane = t & (team - 1), wide = w.width / w.groups;
@@ -117,7 +117,7 @@ __device__ __forceinline__ void gn_coefficient_gradients(const GnParams& p, int 
   const int t = threadIdx.x, c = block * 16 + (t & 15), r0 = t >> 4;
   const int rows = p.N * p.chunks;   // (one-launch kernel: a row an image)
   typedef float v2f __attribute__((ext_vector_type(2)));
-  float a = 0.f, b = 0.f;
+  double a = 0., b = 0.;
   if (c < p.C) {
     const v2f* const at = (const v2f*)p.cpart + c;
     int r = r0;
@@ -137,17 +137,17 @@ __device__ __forceinline__ void gn_coefficient_gradients(const GnParams& p, int 
       b += v[1];
     }
   }
-  s1[t] = a;
-  s2[t] = b;
+  s1[t] = (float)a;
+  s2[t] = (float)b;
   __syncthreads();
   if (t < 16 && c < p.C) {
-    a = b = 0.f;
+    a = b = 0.;
     for (int r = 0; r < 16; ++r) {
       a += s1[r * 16 + t];
       b += s2[r * 16 + t];
     }
-    if (p.dbias) p.dbias[c] = a;
-    if (p.dweight) p.dweight[c] = b;
+    if (p.dbias) p.dbias[c] = (float)a;
+    if (p.dweight) p.dweight[c] = (float)b;
   }
 }
 
@@ -224,11 +224,12 @@ __global__ __launch_bounds__(kGnThreads) void amos_gn_gradient_apply(const GnPar
 __device__ __forceinline__ void gn_slab_totals(const GnParams& p, const GnSlab& w, int parts, float* s1, float* s2, float* e1, float* e2) {
   const int T = (int)blockDim.x, t = threadIdx.x;
   for (int c = t; c < p.ct; c += T) {
-    float a = 0.f, b = 0.f;
+    double a64 = 0., b64 = 0.;
     for (int r = 0; r < parts; ++r) {
-      a += s1[r * p.ct + c];
-      b += s2[r * p.ct + c];
+      a64 += s1[r * p.ct + c];
+      b64 += s2[r * p.ct + c];
     }
+    const float a = (float)a64, b = (float)b64;
     const int at = w.c0 + c;
     if (p.N == 1) {
       if (p.dbias) p.dbias[at] = a;
@@ -317,14 +318,14 @@ __global__ __launch_bounds__(1024) void amos_gn_gradient_held(const GnParams p) 
   if (parts > p.rows) parts = p.rows;
   if (parts > 1) {
     const int c = t % p.ct, part = t / p.ct;
-    float a = 0.f, b = 0.f;
+    double a = 0., b = 0.;
     if (part < parts) {
       for (int r = part; r < p.rows; r += parts) {
         a += s1[r * p.ct + c];
         b += s2[r * p.ct + c];
       }
-      s1[part * p.ct + c] = a;   // (row `part`: read by this thread only)
-      s2[part * p.ct + c] = b;
+      s1[part * p.ct + c] = (float)a;   // (row `part`: read by this thread only)
+      s2[part * p.ct + c] = (float)b;
     }
     __syncthreads();
   } else {
