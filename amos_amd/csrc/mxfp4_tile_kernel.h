@@ -220,7 +220,6 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     }
     if (kt < full) step(kt, I0, I1);
   } else {
-    static_assert(NS == 2, "in phases: this step's stage and the next one's");
     mx_v4i af[2][HA], bf[2][TJ];      // A: by half of the wave tile's rows; B: by sub-step
     int ax[TI], bx[TJ], bx_next[TJ];   // scales: a register serves both sub-steps
     auto read_a = [&](int kt, int stage, auto h, auto ks) {
@@ -263,37 +262,43 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     };
     constexpr int FIRST = TJ * CH / SLOTS;   // copies of part 0
 
-    // the first step whole, of the second one the part that otherwise leaves in the step before
+    // the first NS - 1 steps whole, of the next one the part that otherwise leaves in the step before
 #pragma unroll
-    for (int u = 0; u < CH; ++u) issue_copy(0, 0, u);
-    first_scales();
+    for (int s = 0; s < NS - 1; ++s) {
 #pragma unroll
-    for (int u = 0; u < FIRST; ++u) issue_copy(1 < KT ? 1 : KT - 1, 1, u);
-    if (t.vec_scales) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(FIRST) : "memory");
+      for (int u = 0; u < CH; ++u) issue_copy(s < KT ? s : KT - 1, s, u);
+      if (s == 0) first_scales();
+    }
+#pragma unroll
+    for (int u = 0; u < FIRST; ++u) issue_copy(NS - 1 < KT ? NS - 1 : KT - 1, NS - 1, u);
+    if (t.vec_scales) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((NS - 2) * CH + FIRST) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     read_a(0, 0, I0, I0);
     read_b(0, 0, I0, bx);
 
+    int last = NS - 1;   // the stage whose copies are under way
     for (int kt = 0; kt < full; ++kt) {
-      const int next = st ^ 1;   // the stage whose copies are under way
-      const int ahead = kt + 1 < KT ? kt + 1 : KT - 1, after = kt + 2 < KT ? kt + 2 : KT - 1;
+      const int next = st + 1 == NS ? 0 : st + 1;
+      const int ahead = kt + NS - 1 < KT ? kt + NS - 1 : KT - 1, after = kt + NS < KT ? kt + NS : KT - 1;
       read_a(kt, st, I1, I0);
-      phase(I0, I0, 1, ahead, next);
+      phase(I0, I0, 1, ahead, last);
       issue_scales(kt);
       read_a(kt, st, I0, I1);
       read_b(kt, st, I1, bx);
-      phase(I1, I0, 2, ahead, next);
+      phase(I1, I0, 2, ahead, last);
       read_a(kt, st, I1, I1);
       phase(I0, I1, -1, 0, 0);
-      // all reads of this stage are issued; once they and this wave's copies of the next step are done, meet: behind the
-      // barrier the next stage is whole and this one is free
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      // all reads of this stage are issued; once they and this wave's copies of the next step are done (those of the NS - 2
+      // steps behind it may be under way), meet: behind the barrier the next stage is whole and this one is free.  (Copies
+      // of one width complete in their order.)
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NS - 2) * CH) : "memory");
       asm volatile("s_barrier" ::: "memory");
       read_a(kt + 1, next, I0, I0);   // (behind the last step: read and not used)
       read_b(kt + 1, next, I0, bx_next);
       phase(I1, I1, 0, after, st);
 #pragma unroll
       for (int b = 0; b < TJ; ++b) bx[b] = bx_next[b];
+      last = st;
       st = next;
     }
   }
