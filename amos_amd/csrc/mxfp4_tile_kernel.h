@@ -220,6 +220,7 @@ __global__ __launch_bounds__(64 * WI * WJ) void amos_mx_gemm_tile(const MxTilePa
     }
     if (kt < full) step(kt, I0, I1);
   } else {
+    static_assert(NS == 2, "LDS takes two stages of the one tile that comes here");
     mx_v4i af[2][HA], bf[2][TJ];      // A: by half of the wave tile's rows; B: by sub-step
     int ax[TI], bx[TJ], bx_next[TJ];   // scales: a register serves both sub-steps
     auto read_a = [&](int kt, int stage, auto h, auto ks) {
