@@ -30,7 +30,7 @@ __device__ __forceinline__ unsigned mx_scale_byte(unsigned top_bits) {
 }
 // eight fp32 values -> eight codes.  The conversion instruction divides by the power of two in the
 // exponent field of its scale operand (field 0 = 2^-127), rounds to nearest even and saturates at 6:
-// for finite values exactly the definition above (checked against it over all scales).
+// for finite values exactly the definition above (tests/test_gpu_mxfp4_reach.py goes over all scales).
 __device__ __forceinline__ unsigned mx_encode8(const float* v, unsigned scale_byte) {
   const float s = __builtin_bit_cast(float, scale_byte << 23);
   unsigned c = 0;

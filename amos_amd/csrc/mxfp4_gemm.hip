@@ -214,8 +214,9 @@ static int launch_tile(const MxGemmParams& p, hipStream_t stream) {
 
 // The tile: the one whose rounds of the 256 compute units take the least time.  `one`, `two`: microseconds of a round with
 // one and with two workgroups a unit (the larger tiles' LDS leaves room for one), all at K = 4096; at other K the ratios
-// hold well enough (over 45 shapes of 32 to 8200 rows, 64 to 11000 columns, K 280 to 7700: at most 11 % behind the best of the five, 1 % on the mean).
-//   2048 x 2048 x 2048: 128x128 10.6 us, 64x64 14.5, 256x256 19.6      4096 x 2048 x 4096: 128x256 24.1 us, 128x128 31.8, 256x256 33.1
+// hold well enough (every tile timed on 48 drawn shapes of 34 to 8232 rows, 77 to 10770 columns, K 257 to 7541: the one
+// chosen is at most 7 % behind the best of the five, 0.6 % on the mean).
+//   2048 x 2048 x 2048: 128x128 10.6 us, 64x64 14.5, 256x256 19.6      4096 x 2048 x 4096: 128x256 24.1 us, 128x128 28.5, 256x256 33.6
 //   333 x 1000 x 2050: 32x64 5.4 us, 64x64 6.1                         3000 x 3000 x 1000: 256x256 15.0 us, 128x256 18.4, 128x128 19.4
 // Four stages and a step's fragments read at once let 128x128 in one round wait for neither memory nor LDS (1024 x 4096 x 4096:
 // 15.7 us; three stages with phases 20.3, two workgroups a unit with two stages 19.9).
@@ -256,8 +257,8 @@ static int check_desc(const amos_mxfp4_gemm_desc_t* d) {
 static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
 // Dense rows of A are quantised by the few-rows kernel itself where every workgroup can afford to read and convert all of
-// them: one turn of K a wave, at most 32 KB, no more than three rounds of workgroups.  Else by a launch of its own, codes
-// and scales in the workspace.  (On the GPU, fused / apart: 1 x 4096 x 4096 bf16 5.9 / 5.9 us, 8 x 4096 x 2048 4.7 / 5.3,
+// them: rows of at most 4096 elements (eight waves of a turn each; the sixteen of K = 8192 come out behind), at most 32 KB
+// of them, no more than three rounds of workgroups.  Else by a launch of its own, codes and scales in the workspace.  (On the GPU, fused / apart: 1 x 4096 x 4096 bf16 5.9 / 5.9 us, 8 x 4096 x 2048 4.7 / 5.3,
 // 16 x 1024 x 1024 4.4 / 5.0; 1 x 4096 x 8192 9.3 / 8.5, 4 x 4096 x 4096 fp32, 64 KB, 6.8 / 6.2, 1 x 28672 x 8192 54 / 28.  A launch
 // and an allocation less are 3 us of the host's time as well.)
 static bool quantize_first(const amos_mxfp4_gemm_desc_t* d) {

@@ -10,14 +10,15 @@
 // one 16-byte LDS read; its block's scale is a byte of a register that a 2-byte read fills for both
 // sub-steps and that the matrix instruction takes as it is: no instruction touches a scale.
 // FLAT, where two sets of a step's fragments fit into the registers (all but 256x256): they are read at once, a step ahead
-// (2048 x 2048 x 8192, 128x128 tiles with four stages: 26.7 us; in phases with two or three 34).
+// (2048 x 2048 x 8192, 128x128 tiles with four stages: 25.3 us; in phases, with two, 32.7).
 //
-// 8192^3, fp32 out: 300 us = 3.7 PFLOP/s.  Its matrix instructions alone take 164 us (7.2 PFLOP/s is what they reach on
-// random operands), with their LDS reads 198 - 203, the copies alone 147 (64 KB a K step and compute unit at 28 bytes a
-// cycle, a fifth of it from behind the L2), everything but the stores 238: neither is at its limit by itself (matrix
-// cores 42 % busy, LDS 30 %), the two waves of a SIMD do not fill each other's waits.  The 268 MB of results take the rest.
-// Tried there: four waves of 128x128 (370 us: one wave a SIMD cannot hide its copies), waves as 2x4 (290 where 4x2
-// took 277), stores straight from the registers (301 / 281), copies in two phases (319 / 277).
+// 8192^3, fp32 out: 302 us = 3.6 PFLOP/s (300 - 307 from card to card; bf16 out 293).  Its matrix instructions alone take
+// 164 us (6.7 PFLOP/s; a loop of nothing else reaches 7.0 - 7.2 on random operands, 155 us, and 9.2 on zeros: the clock
+// goes with the power), with their LDS reads 198 - 203, the copies alone 147 (64 KB a K step and compute unit at 28 bytes
+// a cycle, a fifth of it from behind the L2), everything but the stores 238: neither is at its limit by itself (matrix
+// cores 42 % busy, LDS 26 %), the two waves of a SIMD do not fill each other's waits.  The 268 MB of results take the rest.
+// Tried there: four waves of 128x128 (405 us: one wave a SIMD cannot hide its copies), waves as 2x4 (320); on a faster
+// card, on which this kernel took 277 - 281, stores straight from the registers 301, copies in two phases 319.
 // Rows past M / N repeat the last one (their sums are not stored).  K is padded to 128 by the format; an
 // odd number of 128s ends in a half step whose second half is neither read from memory (its lanes fetch
 // the first half again: the row may be the buffer's last) nor multiplied.
@@ -33,7 +34,7 @@ struct MxTileParams {
   MxGemmParams g;
   int tiles_i, tiles_j;
   int vec_scales;       // a row of scales has 16 bytes
-  int stream_out;       // an fp32 C larger than the L2s together: written past them (8192^3: 281 -> 270 us)
+  int stream_out;       // an fp32 C larger than the L2s together: written past them (8192^3: 307 -> 302 us)
 };
 
 // LDS place of a row's 16-byte chunk.  The swizzle goes by the row inside its block of 16, so that the fragments of

@@ -656,7 +656,8 @@ def _dequantize(s, q, d, dtype, out):
 def mxfp4_gemm(a, b, out=None, out_dtype=torch.float32, add=None, bias=None, stream=None):
     """C[M,N] = sum_k A(m,k) B(n,k) (+ bias[N]) (+ add[M,N]); b is an Mxfp4 of shape (N, K), a an
     Mxfp4 of shape (M, K) or a dense matrix [M, K] (fp32, fp16, bf16) that the call quantises the way
-    mxfp4_quantize does.  fp32 accumulation, one rounding to the output's type; `add` may be `out`."""
+    mxfp4_quantize does.  fp32 accumulation, one rounding to the output's type; `add` may be `out`.  No
+    gradient is recorded."""
     if stream is None:
         done = _native.gemm(a, b, out, out_dtype, add, bias)
         if done is not None:
@@ -759,7 +760,7 @@ def group_norm(x, groups, weight=None, bias=None, eps=1e-5, activation=None, lay
     then None / 'relu' / 'silu'.  Statistics and arithmetic are fp32, the result is x's type or
     out_dtype (a convolution's fp32 output can leave at 16 bits for the next one); `out` may be x.  A group
     whose values or squared deviations add up to 2^128 and more (deviations from about 2^64 / sqrt(elements
-    of the group) up), or that holds an infinity or a NaN, is NaN.
+    of the group) up), or that holds an infinity or a NaN, is NaN.  No gradient is recorded.
     stats=True: (y, mean, rstd), both fp32 [N, groups], for group_norm_backward."""
     if stream is None:
         done = _native.group_norm(x, groups, weight, bias, eps, activation, layout, out_dtype, out, stats)
