@@ -33,3 +33,27 @@ def test_misaligned(gpu, shape, groups, dt):
         back = ops.group_norm_backward(moved(dy, j), moved(x, i), moved(mean, k), moved(rstd, i), groups, moved(w, k), moved(b, j), activation="silu")
         for p, q in zip(back, grads):
             assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("over", ["dy", "x"])
+@pytest.mark.parametrize("shape, groups", [((2, 12, 11, 64), 8), ((4, 64, 64, 128), 32), ((1, 66, 65, 30), 3), ((1, 9, 8, 4104), 1)])
+def test_gradient_in_place(gpu, shape, groups, over):
+    """the C call's dx may be dy or x: one launch and two, several chunks and tiles"""
+    import ctypes
+    from amos_amd import _lib, ops
+    lib = _lib.load()
+    w, b = [t.cuda() for t in coefficients(shape[-1], 1)]
+    x, dy = make("nhwc", shape, 3).cuda(), make("nhwc", shape, 4).cuda()
+    _, mean, rstd = ops.group_norm(x, groups, w, b, activation="silu", stats=True)
+    want = ops.group_norm_backward(dy, x, mean, rstd, groups, w, b, activation="silu")
+    n, h, wide, c = shape
+    d = _lib.GroupNormDesc(N=n, C=c, D=1, H=h, W=wide, groups=groups, activation=_lib.AMOS_ACT_SILU, x_dtype=_lib.AMOS_F32, y_dtype=_lib.AMOS_F32,
+                           affine_dtype=_lib.AMOS_F32, layout=_lib.AMOS_LAYOUT_NHWC, eps=1e-5)
+    need = lib.amos_group_norm_workspace_bytes(ctypes.byref(d), 1)
+    ws = torch.empty(need + 8, dtype=torch.uint8, device="cuda")
+    dw, db = torch.empty_like(w), torch.empty_like(b)
+    dx = dict(dy=dy, x=x)[over]
+    at = [t.data_ptr() for t in (dy, x, w, b, mean, rstd, dx, dw, db, ws)]
+    _lib.check(lib.amos_group_norm_backward(ctypes.byref(d), *at, need, torch.cuda.current_stream().cuda_stream))
+    for p, q in zip((dx, dw, db), want):
+        assert torch.equal(p, q)

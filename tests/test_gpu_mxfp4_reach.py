@@ -78,3 +78,17 @@ def test_every_scale(gpu, dtype):
     same_codes(ops.mxfp4_quantize(x.t().contiguous().cuda(), axis=0), want)
     for back in DTYPES:
         assert torch.equal(ops.mxfp4_dequantize(q, back).cpu(), ref.values(*want, 96).float().to(back))
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+def test_more_than_31_bits_of_results(gpu, out):
+    """a product of 2^31 and more results: its first, middle and last rows"""
+    from amos_amd import ops
+    M, N, K = 46400, 46500, 96
+    g = torch.Generator().manual_seed(3)
+    a, b = ref.random_codes(g, M, K), ref.random_codes(g, N, K)
+    assert M * N > 1 << 31
+    c = ops.mxfp4_gemm(put(a, K), put(b, K), out_dtype=out)
+    av, bv = ref.values(*a, K), ref.values(*b, K)
+    rows = torch.cat([torch.arange(3), torch.arange(23100, 23110), torch.arange(M - 300, M, 7), torch.tensor([M - 1])])
+    assert torch.equal(c[rows.cuda()].cpu(), (av[rows] @ bv.t()).float().to(out))
