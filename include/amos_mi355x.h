@@ -429,8 +429,8 @@ int amos_mxfp4_gemm(const amos_mxfp4_gemm_desc_t* desc, const amos_mxfp4_epilogu
  * whose values or squared deviations add up to 2^128 and more (deviations from about 2^64 / sqrt(elements
  * of the group) up), or that holds an infinity or a NaN, has rstd and results of NaN.  y may be x where
  * their types agree.
- * Gradient (with the forward's mean and rstd): dx of x's type, dweight and dbias fp32 [C] or NULL; dy has
- * y's type.  dx may be dy or x where the types agree.  rstd^2 is formed in fp32: rstd below 2^63.  Results do not depend on the order in which
+ * Gradient (with the forward's mean and rstd): dx of x's type, dweight and dbias fp32 [C] or NULL (added in
+ * 64 bits from where a workgroup's pixels meet); dy has y's type.  dx may be dy or x where the types agree.  rstd^2 is formed in fp32: rstd below 2^63.  Results do not depend on the order in which
  * workgroups run.
  * The reference leaves normalisation layers to its fallback scheduler
  * (python/tvm/tensor_graph/core/auto_schedule/auto_schedule.py:1090-1160).

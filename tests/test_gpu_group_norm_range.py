@@ -48,3 +48,16 @@ def test_large_equal_values(gpu, shape, value):
     y, mean, rstd = ops.group_norm(torch.full(shape, value, device="cuda"), 2, w, b, stats=True)
     assert (mean == value).all() and torch.allclose(rstd, torch.full_like(rstd, 1e-5 ** -0.5), rtol=1e-6)
     assert torch.equal(y, b.expand(shape))
+
+
+@pytest.mark.parametrize("shape", [(1, 12, 12, 64), (3, 12, 12, 64), (2, 64, 64, 256), (1, 66, 65, 30)])
+def test_sums_of_coefficient_gradients_that_cancel(gpu, shape):
+    """three neighbouring pixels, which three rows of threads take, with dy = 2^26, 1 and -2^26 and h = 1: every share is
+    exact, and their sum is 1 where it is taken in more than fp32's 24 bits"""
+    from amos_amd import ops
+    c = shape[-1]
+    dy = torch.zeros(shape, device="cuda")
+    dy[0, 0, 0], dy[0, 0, 1], dy[0, 0, 2] = 2.0 ** 26, 1.0, -2.0 ** 26
+    zero, one = torch.zeros(shape[0], 2, device="cuda"), torch.ones(shape[0], 2, device="cuda")
+    dx, dw, db = ops.group_norm_backward(dy, torch.ones(shape, device="cuda"), zero, one, 2, torch.ones(c, device="cuda"), torch.zeros(c, device="cuda"))
+    assert (dw == 1).all() and (db == 1).all() and dx.isfinite().all()
